@@ -59,7 +59,11 @@ typedef struct { const int64_t* counter; uint64_t seed; float p; const int32_t* 
 #define M3D_IO_A32 0x2000
 #define M3D_IO_C32 0x4000
 
-#define M3D_ABI_VERSION 18
+#define M3D_ABI_VERSION 19
+/* element types of the entry points that take one (M3D_TYPE_*) */
+#define M3D_TYPE_F32 0
+#define M3D_TYPE_BF16 1
+#define M3D_TYPE_F16 2
 #define M3D_ADAM_STATE_WORDS 66
 #define M3D_CE_ACC_DOUBLES 516
 int m3d_abi_version(void);
@@ -513,6 +517,65 @@ int m3d_dropout(const float* x, float* y, int64_t n, float p, const int64_t* cou
 /* start of a training step: zero-fill of `nbytes` (multiple of 16, 16-byte aligned: the step's accumulation arena) and
  * counters[0 .. ncounters) += 1 (the BatchNorm layers' num_batches_tracked, int64) in one launch */
 int m3d_zero_bump(void* buf, int64_t nbytes, int64_t* counters, int32_t ncounters, void* stream);
+
+
+/* ---- layer norm ------------------------------------------------------------------------------------------------
+ * torch.nn.LayerNorm over the last dimension, with the LeakyReLU that follows a SharedMLP's normalisation
+ * (pyg_randla_net.py:92-109 has batch norm there; PyG's MLP takes norm="layer_norm"):
+ *   mean, var over the row;  z = (x - mean) / sqrt(var + eps) * w + b;  y = z > 0 ? z : slope * z   (slope = 1: none)
+ * x: [rows, cols], row stride ldx elements (0: the same row again); y contiguous; type: of x and y, wtype: of w and b
+ * (nullable: ones, zeros).  mean, rstd: fp32 [rows] kept for the backward pass (both or neither).  Any cols >= 1; up to
+ * 16 384 a row is read once. */
+int m3d_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int64_t rows, int32_t cols, int32_t type,
+                       int32_t wtype, float eps, float slope, void* y, float* mean, float* rstd, void* stream);
+size_t m3d_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t type);
+/* dx [rows, cols] contiguous, dw, db [cols] of wtype (each nullable: not wanted).  dy: row stride lddy.  ws: the workspace
+ * (partial sums of dw and db; not needed when both are null).  No atomics: the same inputs give the same bits. */
+int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* b,
+                       const float* mean, const float* rstd, int64_t rows, int32_t cols, int32_t type, int32_t wtype,
+                       float slope, void* dx, void* dw, void* db, void* ws, void* stream);
+
+/* ---- many tensors at once: gradient norm, clipping, AdamW -----------------------------------------------------
+ * The reference trains through Lightning, whose gradient_clip_val and torch optimizers loop over the parameter tensors.
+ * `grads`, `numel`, `types` (and the arrays of M3DAdamW) are HOST arrays of `count` entries read during the call: device
+ * pointer of a contiguous tensor (grads: NULL = the tensor has no gradient; aligned to its element, no more), number of
+ * elements, type (M3D_TYPE_*).  Any count; the pointers travel as kernel arguments, 152 tensors a launch. */
+#define M3D_GRAD_NORM_PARTS 1024
+/* parts (device fp64 [M3D_GRAD_NORM_PARTS]) <- partial sums of g^2 over all tensors, *nparts (host) <- how many of them are
+ * written: the norm is the root of their sum, which m3d_clip_grads and m3d_adamw_step take themselves.  No atomics: the
+ * same gradients give the same bits. */
+int m3d_grad_norm(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count, double* parts,
+                  int32_t* nparts, void* stream);
+/* g *= min(1, max_norm / (norm + 1e-6)) in place (torch.nn.utils.clip_grad_norm_); norm_out (nullable, device fp32) <- norm.
+ * A norm that is not finite behaves as in torch: infinite -> zeros (and NaN for the infinite ones), NaN -> NaN. */
+int m3d_clip_grads(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count, const double* parts,
+                   int32_t nparts, double max_norm, float* norm_out, void* stream);
+/* One AdamW update (torch.optim.AdamW, amsgrad=False, maximize=False) of `count` tensors.
+ *   exp_avg, exp_avg_sq  the moments of ALL tensors, in blocks of 256 elements: tensor i's slice starts at 256 times the sum of
+ *                        ceil(numel / 256) over the tensors in front of it.  state_bits 32: fp32; 8: one byte an element with
+ *                        one fp32 per block in scale_avg / scale_avg_sq:
+ *                          first moment   e4m3(code) / 256 * scale, scale = the block's largest magnitude (code 0x7f: NaN)
+ *                          second moment  2^((code >> 3) - 31) * (1 + (code & 7) / 8) * scale, code 0 = zero, 255 = not finite;
+ *                                         a positive value never becomes zero
+ *                        both to nearest even of b1 * m + (1 - b1) * g and b2 * v + (1 - b2) * (g * g), each operation in 64
+ *                        bits, over the scale; a scale under 2^-126 becomes zero, and the block's codes with it.
+ *   state                [M3D_ADAM_STATE_WORDS] x 4 bytes on the device: [0] fp32 count of updates, the rest tickets (zero)
+ *   missed               device int32 [count]: updates in which tensor i had no gradient (its own count is state[0] - missed)
+ *   parts, nparts        of m3d_grad_norm: the gradient is clipped to max_norm on the way in (the tensor keeps its values), and
+ *                        an update whose norm is not finite is not taken; NULL: neither.  norm_out: as m3d_clip_grads
+ *   lr_dev               optional device fp32 [1] in place of lr */
+typedef struct {
+  void* const* params; void* const* grads; const int64_t* numel; const int32_t* types; int32_t count; int32_t state_bits;
+  void* exp_avg; void* exp_avg_sq; float* scale_avg; float* scale_avg_sq; float* state; int32_t* missed;
+  const double* parts; int32_t nparts; double max_norm; float* norm_out; const float* lr_dev;
+  double lr; double beta1; double beta2; double eps; double weight_decay;
+} M3DAdamW;
+int m3d_adamw_step(const M3DAdamW* args, void* stream);
+/* `blocks` blocks of 8-bit moments (layout above) -> fp32, and back (the same codes and scales for decoded values). */
+int m3d_moments_decode(const void* exp_avg, const void* exp_avg_sq, const float* scale_avg, const float* scale_avg_sq,
+                       float* avg_out, float* avg_sq_out, int64_t blocks, void* stream);
+int m3d_moments_encode(const float* avg, const float* avg_sq, void* exp_avg, void* exp_avg_sq, float* scale_avg,
+                       float* scale_avg_sq, int64_t blocks, void* stream);
 
 #ifdef __cplusplus
 }

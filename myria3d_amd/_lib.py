@@ -97,6 +97,14 @@ SIGNATURES = {
     "m3d_ce_loss_fwd": (_i32, [_p, _i64, _p, _i64, _i32, _i64, _p, _p, _p, _i32, _p]),
     "m3d_ce_loss_bwd": (_i32, [_p, _i64, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p]),
     "m3d_adam_step": (_i32, [_p, _p, _p, _p, _p, _p, _f32, _f32, _f32, _f32, _f32, _f32, _i32, _i64, _p]),
+    "m3d_layer_norm_fwd": (_i32, [_p, _i64, _p, _p, _i64, _i32, _i32, _i32, _f32, _f32, _p, _p, _p, _p]),
+    "m3d_layer_norm_bwd_workspace_bytes": (C.c_size_t, [_i64, _i32, _i32]),
+    "m3d_layer_norm_bwd": (_i32, [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _f32, _p, _p, _p, _p, _p]),
+    "m3d_grad_norm": (_i32, [_p, _p, _p, _i32, _p, _p, _p]),
+    "m3d_clip_grads": (_i32, [_p, _p, _p, _i32, _p, _i32, C.c_double, _p, _p]),
+    "m3d_adamw_step": (_i32, [_p, _p]),
+    "m3d_moments_decode": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p]),
+    "m3d_moments_encode": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p]),
     "m3d_zero_bump": (_i32, [_p, _i64, _p, _i32, _p]),
     "m3d_dropout": (_i32, [_p, _p, _i64, _f32, _p, C.c_uint64, _p]),
 }
@@ -115,7 +123,17 @@ class M3DBnOnLoad(C.Structure):
                 ("invstd", C.c_void_p), ("act", C.c_int32), ("slope", C.c_float), ("y", C.c_void_p)]
 
 
-ABI_VERSION = 18  # M3D_ABI_VERSION in include/m3d_hip.h
+class M3DAdamW(C.Structure):
+    """``M3DAdamW`` of include/m3d_hip.h (read by the library on the host, at call time)."""
+    _fields_ = [("params", C.c_void_p), ("grads", C.c_void_p), ("numel", C.c_void_p), ("types", C.c_void_p),
+                ("count", C.c_int32), ("state_bits", C.c_int32), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("scale_avg", C.c_void_p), ("scale_avg_sq", C.c_void_p), ("state", C.c_void_p), ("missed", C.c_void_p),
+                ("parts", C.c_void_p), ("nparts", C.c_int32), ("max_norm", C.c_double), ("norm_out", C.c_void_p),
+                ("lr_dev", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("weight_decay", C.c_double)]
+
+
+ABI_VERSION = 19  # M3D_ABI_VERSION in include/m3d_hip.h
 
 _ERRORS = {-1: "invalid argument", -2: "unsupported shape", -3: "kernel launch failure"}
 

@@ -1,0 +1,522 @@
+// Layer norm over the last dimension, forward and backward (gfx950).
+//
+//   mu = mean_c x,  var = mean_c (x - mu)^2,  r = 1 / sqrt(var + eps),  xh = (x - mu) r,  z = xh w + b,  y = z > 0 ? z : slope z
+//   g = dy (z > 0 ? 1 : slope);  dx = r (g w - mean_c(g w) - xh mean_c(g w xh));  dw = sum_rows g xh;  db = sum_rows g
+//
+// (slope = 1: no activation.)  About 8 operations an element forward and 20 backward against 4 to 12 bytes: the memory bounds
+// both, so a row is read ONCE and stays in registers — forward for the mean, the squared deviations from it (two steps: a large
+// common offset costs no digits) and the result, backward for the two row sums and the result.
+//
+// A row belongs to TPR lanes, each with NE vectors of 16 bytes (4 fp32 or 8 half-precision elements) and, where the width is not
+// a multiple of a vector, one element of the rest.  Up to 64 lanes the row sits inside a wave (narrow rows: several rows a wave,
+// sums by lane swaps, no LDS); above, a workgroup of 128 to 1 024 threads takes a row (sums over its waves through LDS).  The
+// columns of a lane are the same for every row it meets: w and b are read once per lane, and the backward pass keeps dw and db of
+// its columns in registers over all its rows.  At the end the waves of a workgroup are added up through LDS in a fixed order, the
+// workgroups leave one row of partial sums each, and a second kernel adds these in 64 bits: no atomics, the same bits every time.
+// Vectors are loaded with the alignment of their element, so rows of any stride take this path.
+#include "m3d_common.h"
+#include "../../include/m3d_hip.h"
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short h8u __attribute__((ext_vector_type(8), aligned(2)));
+
+struct NormArgs {
+  const void *x, *dy, *w, *b;
+  void *y, *dx;
+  float *mean, *rstd;   // forward: written (nullable); backward: read
+  float* parts;         // backward: [gridDim.x][2][cols], or null: no weight gradients
+  int64_t rows, ldx, lddy;
+  int32_t cols, wtype;  // type of w and b
+  float eps, slope, inv;
+};
+
+template <int TYPE> struct Vec { static constexpr int N = TYPE == M3D_TYPE_F32 ? 4 : 8; };
+template <int TYPE>
+__device__ __forceinline__ float el_load(const void* base, int64_t e) {
+  if constexpr (TYPE == M3D_TYPE_F32) return ((const float*)base)[e];
+  else if constexpr (TYPE == M3D_TYPE_BF16) return bf16_to_f32(((const unsigned short*)base)[e]);
+  else return (float)((const _Float16*)base)[e];
+}
+template <int TYPE>
+__device__ __forceinline__ void el_store(void* base, int64_t e, float v) {
+  if constexpr (TYPE == M3D_TYPE_F32) ((float*)base)[e] = v;
+  else if constexpr (TYPE == M3D_TYPE_BF16) ((unsigned short*)base)[e] = f32_to_bf16(v);
+  else ((_Float16*)base)[e] = (_Float16)v;
+}
+template <int TYPE>
+__device__ __forceinline__ void vec_load(const void* base, int64_t e, float* v) {
+  if constexpr (TYPE == M3D_TYPE_F32) {
+    const f4u t = *(const f4u*)((const float*)base + e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = t[j];
+  } else {
+    const h8u t = *(const h8u*)((const unsigned short*)base + e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned short u = t[j];
+      v[j] = TYPE == M3D_TYPE_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
+    }
+  }
+}
+template <int TYPE>
+__device__ __forceinline__ void vec_store(void* base, int64_t e, const float* v) {
+  if constexpr (TYPE == M3D_TYPE_F32) {
+    f4u t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = v[j];
+    *(f4u*)((float*)base + e) = t;
+  } else {
+    h8u t;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      if constexpr (TYPE == M3D_TYPE_BF16) {
+        const unsigned p = pack_bf16(v[j], v[j + 1]);
+        t[j] = (unsigned short)(p & 0xffffu);
+        t[j + 1] = (unsigned short)(p >> 16);
+      } else {
+        t[j] = __builtin_bit_cast(unsigned short, (_Float16)v[j]);
+        t[j + 1] = __builtin_bit_cast(unsigned short, (_Float16)v[j + 1]);
+      }
+    }
+    *(h8u*)((unsigned short*)base + e) = t;
+  }
+}
+__device__ __forceinline__ float w_load(const void* base, int64_t e, int type, float none) {
+  if (!base) return none;
+  return type == M3D_TYPE_F32 ? el_load<M3D_TYPE_F32>(base, e) : type == M3D_TYPE_BF16 ? el_load<M3D_TYPE_BF16>(base, e) : el_load<M3D_TYPE_F16>(base, e);
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+// sum over groups of TPR lanes, in every lane of the group
+template <int TPR>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp_f<0xB1>(v);                          // quad_perm [1,0,3,2]
+  v += dpp_f<0x4E>(v);                          // quad_perm [2,3,0,1]
+  v += dpp_f<0x141>(v);                         // row_half_mirror: 8 lanes
+  if constexpr (TPR >= 16) v += dpp_f<0x140>(v);  // row_mirror: 16 lanes
+  float a, b;
+  if constexpr (TPR >= 32) { xgroup_pair16(v, a, b); v = a + b; }
+  if constexpr (TPR >= 64) { xgroup_pair32(v, a, b); v = a + b; }
+  return v;
+}
+// the lanes at the same place of every group of TPR lanes of a wave, added up
+template <int TPR>
+__device__ __forceinline__ float across_groups(float v) {
+  float a, b;
+  if constexpr (TPR <= 32) { xgroup_pair32(v, a, b); v = a + b; }
+  if constexpr (TPR <= 16) { xgroup_pair16(v, a, b); v = a + b; }
+  if constexpr (TPR <= 8) v += dpp_f<0x128>(v);  // row_ror:8
+  return v;
+}
+// a row over a whole workgroup: wave sums through LDS; `flip` alternates the two halves of red, so that one barrier a sum is enough
+template <int S>
+__device__ __forceinline__ void wg_sums(float (&v)[S], float (*red)[16][S], int& flip) {
+  const int waves = blockDim.x >> 6;
+#pragma unroll
+  for (int s = 0; s < S; ++s) v[s] = group_sum<64>(v[s]);
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) red[flip][threadIdx.x >> 6][s] = v[s];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < S; ++s) v[s] = 0.f;
+  for (int i = 0; i < waves; ++i) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) v[s] += red[flip][i][s];
+  }
+  flip ^= 1;
+}
+
+// TPR = 0: a workgroup a row (TPR = 1 024: one of that many threads, whose lanes have half the registers)
+#define NORM_THREADS(TPR) ((TPR) == 0 ? 512 : (TPR) == 1024 ? 1024 : 256)
+template <int TYPE, int TPR, int NE>
+__global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const NormArgs A) {
+  constexpr int V = Vec<TYPE>::N;
+  constexpr bool IN = TPR > 0 && TPR <= 64;  // the row sits inside a wave
+  constexpr int G = IN ? TPR : 64;
+  __shared__ float red[2][16][1];
+  const int lanes = IN ? G : blockDim.x, lane = IN ? threadIdx.x & (G - 1) : threadIdx.x;
+  const int nv = A.cols / V, rest = nv * V + lane;  // full vectors of a row; this lane's element behind them
+  const bool has_rest = rest < A.cols;
+  float w[NE * V + 1], b[NE * V + 1];
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (lane + i * lanes) * V + j;
+      w[i * V + j] = c < nv * V ? w_load(A.w, c, A.wtype, 1.f) : 0.f;
+      b[i * V + j] = c < nv * V ? w_load(A.b, c, A.wtype, 0.f) : 0.f;
+    }
+  w[NE * V] = has_rest ? w_load(A.w, rest, A.wtype, 1.f) : 0.f;
+  b[NE * V] = has_rest ? w_load(A.b, rest, A.wtype, 0.f) : 0.f;
+  const int per = IN ? 256 / G : 1;  // rows a workgroup holds at a time
+  int flip = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < A.rows; r0 += (int64_t)gridDim.x * per) {
+    const int64_t row = r0 + (IN ? threadIdx.x / G : 0);
+    const bool on = row < A.rows;  // (lanes of a row that is not there take part in the lane swaps)
+    const int64_t xo = row * A.ldx;
+    float x[NE * V + 1];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int q = lane + i * lanes;
+      if (on && q < nv) vec_load<TYPE>(A.x, xo + q * V, &x[i * V]);
+      else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i * V + j] = 0.f;
+      }
+    }
+    x[NE * V] = on && has_rest ? el_load<TYPE>(A.x, xo + rest) : 0.f;
+    float s[1] = {x[NE * V]};
+#pragma unroll
+    for (int e = 0; e < NE * V; ++e) s[0] += x[e];
+    if constexpr (IN) s[0] = group_sum<G>(s[0]);
+    else wg_sums<1>(s, red, flip);
+    const float mean = s[0] / (float)A.cols;  // (a division: the mean of a constant row is that constant)
+    float q2[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = lane + i * lanes < nv ? x[i * V + j] - mean : 0.f;
+        x[i * V + j] = d;
+        q2[0] = fmaf(d, d, q2[0]);
+      }
+    x[NE * V] = has_rest ? x[NE * V] - mean : 0.f;
+    q2[0] = fmaf(x[NE * V], x[NE * V], q2[0]);
+    if constexpr (IN) q2[0] = group_sum<G>(q2[0]);
+    else wg_sums<1>(q2, red, flip);
+    const float rstd = 1.f / sqrtf(q2[0] * A.inv + A.eps);
+    if (!on) continue;
+    if (lane == 0 && A.mean) { A.mean[row] = mean; A.rstd[row] = rstd; }
+    const int64_t yo = row * A.cols;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int q = lane + i * lanes;
+      if (q < nv) {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float z = fmaf(x[i * V + j] * rstd, w[i * V + j], b[i * V + j]);
+          o[j] = z > 0.f ? z : z * A.slope;
+        }
+        vec_store<TYPE>(A.y, yo + q * V, o);
+      }
+    }
+    if (has_rest) {
+      const float z = fmaf(x[NE * V] * rstd, w[NE * V], b[NE * V]);
+      el_store<TYPE>(A.y, yo + rest, z > 0.f ? z : z * A.slope);
+    }
+  }
+}
+
+template <int TYPE, int TPR, int NE, bool ACT>
+__global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const NormArgs A) {
+  constexpr int V = Vec<TYPE>::N, E = NE * V + 1;
+  constexpr bool IN = TPR > 0 && TPR <= 64;  // the row sits inside a wave
+  constexpr int G = IN ? TPR : 64;
+  __shared__ float red[2][16][2];
+  extern __shared__ float sums[];  // IN: [2][cols], the workgroup's dw and db
+  const int lanes = IN ? G : blockDim.x, lane = IN ? threadIdx.x & (G - 1) : threadIdx.x;
+  const int nv = A.cols / V, rest = nv * V + lane;
+  const bool has_rest = rest < A.cols;
+  float w[E], b[ACT ? E : 1], dw[E], db[E];  // (b only to find the sign of z again)
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (lane + i * lanes) * V + j;
+      w[i * V + j] = c < nv * V ? w_load(A.w, c, A.wtype, 1.f) : 0.f;
+      if constexpr (ACT) b[i * V + j] = c < nv * V ? w_load(A.b, c, A.wtype, 0.f) : 0.f;
+    }
+  w[E - 1] = has_rest ? w_load(A.w, rest, A.wtype, 1.f) : 0.f;
+  if constexpr (ACT) b[E - 1] = has_rest ? w_load(A.b, rest, A.wtype, 0.f) : 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
+  const int per = IN ? 256 / G : 1;
+  int flip = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < A.rows; r0 += (int64_t)gridDim.x * per) {
+    const int64_t row = r0 + (IN ? threadIdx.x / G : 0);
+    const bool on = row < A.rows;
+    const int64_t xo = row * A.ldx, go = row * A.lddy;
+    float x[E], g[E];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int q = lane + i * lanes;
+      if (on && q < nv) {
+        vec_load<TYPE>(A.x, xo + q * V, &x[i * V]);
+        vec_load<TYPE>(A.dy, go + q * V, &g[i * V]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i * V + j] = g[i * V + j] = 0.f;
+      }
+    }
+    x[E - 1] = on && has_rest ? el_load<TYPE>(A.x, xo + rest) : 0.f;
+    g[E - 1] = on && has_rest ? el_load<TYPE>(A.dy, go + rest) : 0.f;
+    const float mean = on ? A.mean[row] : 0.f, rstd = on ? A.rstd[row] : 0.f;
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool there = e == E - 1 ? on && has_rest : on && lane + (e / V) * lanes < nv;
+      const float xh = there ? (x[e] - mean) * rstd : 0.f;  // (a lane past the end adds nothing, also where the mean is not finite)
+      if constexpr (ACT) g[e] = fmaf(xh, w[e], b[e]) > 0.f ? g[e] : g[e] * A.slope;
+      const float gw = g[e] * w[e];
+      s[0] += gw;
+      s[1] = fmaf(gw, xh, s[1]);
+      dw[e] = fmaf(g[e], xh, dw[e]);
+      db[e] += g[e];
+      x[e] = xh;
+      g[e] = gw;
+    }
+    if constexpr (IN) {
+      s[0] = group_sum<G>(s[0]);
+      s[1] = group_sum<G>(s[1]);
+    } else wg_sums<2>(s, red, flip);
+    if (!on || !A.dx) continue;
+    const float m0 = s[0] * A.inv, m1 = s[1] * A.inv;
+    const int64_t yo = row * A.cols;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int q = lane + i * lanes;
+      if (q < nv) {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = rstd * (g[i * V + j] - m0 - x[i * V + j] * m1);
+        vec_store<TYPE>(A.dx, yo + q * V, o);
+      }
+    }
+    if (has_rest) el_store<TYPE>(A.dx, yo + rest, rstd * (g[E - 1] - m0 - x[E - 1] * m1));
+  }
+  if (!A.parts) return;
+  float* out = A.parts + (int64_t)blockIdx.x * 2 * A.cols;
+  if constexpr (IN) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      dw[e] = across_groups<G>(dw[e]);
+      db[e] = across_groups<G>(db[e]);
+    }
+    const int wave = threadIdx.x >> 6;
+    for (int k = 0; k < 4; ++k) {  // one wave after the other: the same order every time
+      if (wave == k && (threadIdx.x & 63) < G) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int c = e == E - 1 ? rest : (lane + (e / V) * lanes) * V + e % V;
+          if (e == E - 1 ? has_rest : c < nv * V) {
+            sums[c] = k ? sums[c] + dw[e] : dw[e];
+            sums[A.cols + c] = k ? sums[A.cols + c] + db[e] : db[e];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < 2 * A.cols; c += 256) out[c] = sums[c];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = e == E - 1 ? rest : (lane + (e / V) * lanes) * V + e % V;
+      if (e == E - 1 ? has_rest : c < nv * V) { out[c] = dw[e]; out[A.cols + c] = db[e]; }
+    }
+  }
+}
+
+// Rows too wide for the registers of 1 024 threads: the row is read again (from cache) for every step.
+template <int TYPE>
+__global__ __launch_bounds__(1024) void layer_norm_wide_kernel(const NormArgs A) {
+  __shared__ float red[2][16][1];
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
+    const int64_t xo = row * A.ldx;
+    float s[1] = {0.f}, q2[1] = {0.f};
+    for (int c = threadIdx.x; c < A.cols; c += 1024) s[0] += el_load<TYPE>(A.x, xo + c);
+    wg_sums<1>(s, red, flip);
+    const float mean = s[0] / (float)A.cols;  // (a division: the mean of a constant row is that constant)
+    for (int c = threadIdx.x; c < A.cols; c += 1024) {
+      const float d = el_load<TYPE>(A.x, xo + c) - mean;
+      q2[0] = fmaf(d, d, q2[0]);
+    }
+    wg_sums<1>(q2, red, flip);
+    const float rstd = 1.f / sqrtf(q2[0] * A.inv + A.eps);
+    if (threadIdx.x == 0 && A.mean) { A.mean[row] = mean; A.rstd[row] = rstd; }
+    for (int c = threadIdx.x; c < A.cols; c += 1024) {
+      const float z = fmaf((el_load<TYPE>(A.x, xo + c) - mean) * rstd, w_load(A.w, c, A.wtype, 1.f), w_load(A.b, c, A.wtype, 0.f));
+      el_store<TYPE>(A.y, row * A.cols + c, z > 0.f ? z : z * A.slope);
+    }
+  }
+}
+// (dw and db: a workgroup owns a run of rows AND walks all columns, adding to its own row of partial sums)
+template <int TYPE>
+__global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const NormArgs A) {
+  __shared__ float red[2][16][2];
+  int flip = 0;
+  float* out = A.parts ? A.parts + (int64_t)blockIdx.x * 2 * A.cols : nullptr;
+  bool first = true;
+  for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
+    const int64_t xo = row * A.ldx, go = row * A.lddy;
+    const float mean = A.mean[row], rstd = A.rstd[row];
+    float s[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < A.cols; c += 1024) {
+      const float xh = (el_load<TYPE>(A.x, xo + c) - mean) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
+      float g = el_load<TYPE>(A.dy, go + c);
+      if (A.slope != 1.f) g = fmaf(xh, w, w_load(A.b, c, A.wtype, 0.f)) > 0.f ? g : g * A.slope;
+      s[0] += g * w;
+      s[1] = fmaf(g * w, xh, s[1]);
+      if (out) {
+        out[c] = first ? g * xh : fmaf(g, xh, out[c]);
+        out[A.cols + c] = first ? g : out[A.cols + c] + g;
+      }
+    }
+    first = false;
+    wg_sums<2>(s, red, flip);
+    if (!A.dx) continue;
+    const float m0 = s[0] * A.inv, m1 = s[1] * A.inv;
+    for (int c = threadIdx.x; c < A.cols; c += 1024) {
+      const float xh = (el_load<TYPE>(A.x, xo + c) - mean) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
+      float g = el_load<TYPE>(A.dy, go + c);
+      if (A.slope != 1.f) g = fmaf(xh, w, w_load(A.b, c, A.wtype, 0.f)) > 0.f ? g : g * A.slope;
+      el_store<TYPE>(A.dx, row * A.cols + c, rstd * (g * w - m0 - xh * m1));
+    }
+  }
+}
+
+// dw and db: the partial rows added up in 64 bits.  16 columns (64 bytes) a workgroup, 64 of its threads to a column.
+__global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __restrict__ parts, int nparts, int cols, int wtype,
+                                                                void* __restrict__ dw, void* __restrict__ db) {
+  __shared__ double red[64][17];
+  const int tc = threadIdx.x & 15, tr = threadIdx.x >> 4, c = blockIdx.x * 16 + tc;
+  const int64_t ld = 2 * (int64_t)cols;
+  double s = 0.0;
+  if (c < ld) {
+    int p = tr;
+    for (; p + 3 * 64 < nparts; p += 4 * 64) {
+      float v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = parts[(p + u * 64) * ld + c];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += (double)v[u];
+    }
+    for (; p < nparts; p += 64) s += (double)parts[p * ld + c];
+  }
+  red[tr][tc] = s;
+  __syncthreads();
+  for (int h = 32; h > 0; h >>= 1) {
+    if (tr < h) red[tr][tc] += red[tr + h][tc];
+    __syncthreads();
+  }
+  if (tr == 0 && c < ld) {
+    void* out = c < cols ? dw : db;
+    const int k = c < cols ? c : c - cols;
+    const float v = (float)red[0][tc];
+    if (!out) return;
+    if (wtype == M3D_TYPE_F32) el_store<M3D_TYPE_F32>(out, k, v);
+    else if (wtype == M3D_TYPE_BF16) el_store<M3D_TYPE_BF16>(out, k, v);
+    else el_store<M3D_TYPE_F16>(out, k, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+// How a row is laid over lanes: as few lanes as hold it in 16 elements each (fewer lanes: fewer steps in the sums and fewer idle
+// ones; more elements than 16 would cost the backward pass its occupancy).  tpr = 0 with threads > 0: a workgroup a row.
+struct NormShape { int tpr, ne, threads; };
+static NormShape norm_shape(int32_t cols, int32_t type) {
+  const int V = type == M3D_TYPE_F32 ? 4 : 8, most = 16 / V, nv = cols / V;
+  for (int tpr = 8; tpr <= 64; tpr *= 2)
+    for (int ne = 1; ne <= most; ne *= 2)
+      if (nv <= tpr * ne) return {tpr, ne, 256};
+  for (int threads = 128; threads <= 1024; threads *= 2)
+    for (int ne = 1; ne <= most; ne *= 2)
+      if (nv <= threads * ne) return {0, ne, threads};
+  return {0, 0, 1024};
+}
+static int norm_per(const NormShape& s) { return s.tpr ? 256 / s.tpr : 1; }
+// workgroups: enough for 16 waves on each of the 256 compute units, never more than there is work
+static int64_t norm_grid(const NormShape& s, int64_t rows) {
+  const int64_t most = 256 * (s.threads >= 1024 ? 2 : 1024 / s.threads), need = m3d_cdiv(rows, norm_per(s));
+  return need < most ? need : most;
+}
+
+template <int TYPE, int TPR>
+static void launch_norm(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, size_t lds, hipStream_t st) {
+#define NORM_LAUNCH(NE)                                                                                                                       \
+  if (!bwd) hipLaunchKernelGGL((layer_norm_kernel<TYPE, TPR, NE>), dim3((unsigned)grid), dim3(s.threads), 0, st, A);                          \
+  else if (A.slope != 1.f) hipLaunchKernelGGL((layer_norm_bwd_kernel<TYPE, TPR, NE, true>), dim3((unsigned)grid), dim3(s.threads), lds, st, A); \
+  else hipLaunchKernelGGL((layer_norm_bwd_kernel<TYPE, TPR, NE, false>), dim3((unsigned)grid), dim3(s.threads), lds, st, A)
+  if (s.ne == 1) { NORM_LAUNCH(1); }
+  else if (s.ne == 2) { NORM_LAUNCH(2); }
+  else if constexpr (TYPE == M3D_TYPE_F32) { NORM_LAUNCH(4); }
+#undef NORM_LAUNCH
+}
+template <int TYPE>
+static void launch_norm_type(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, hipStream_t st) {
+  const size_t lds = bwd && s.tpr && A.parts ? 2 * sizeof(float) * (size_t)A.cols : 0;
+  if (s.ne == 0) {
+    if (bwd) hipLaunchKernelGGL(layer_norm_wide_bwd_kernel<TYPE>, dim3((unsigned)grid), dim3(1024), 0, st, A);
+    else hipLaunchKernelGGL(layer_norm_wide_kernel<TYPE>, dim3((unsigned)grid), dim3(1024), 0, st, A);
+    return;
+  }
+  switch (s.tpr) {
+    case 8: launch_norm<TYPE, 8>(A, s, grid, bwd, lds, st); break;
+    case 16: launch_norm<TYPE, 16>(A, s, grid, bwd, lds, st); break;
+    case 32: launch_norm<TYPE, 32>(A, s, grid, bwd, lds, st); break;
+    case 64: launch_norm<TYPE, 64>(A, s, grid, bwd, lds, st); break;
+    default:
+      if (s.threads > 512) launch_norm<TYPE, 1024>(A, s, grid, bwd, lds, st);
+      else launch_norm<TYPE, 0>(A, s, grid, bwd, lds, st);
+  }
+}
+static int launch_norm_any(const NormArgs& A, const NormShape& s, int64_t grid, int32_t type, bool bwd, hipStream_t st) {
+  if (type == M3D_TYPE_F32) launch_norm_type<M3D_TYPE_F32>(A, s, grid, bwd, st);
+  else if (type == M3D_TYPE_BF16) launch_norm_type<M3D_TYPE_BF16>(A, s, grid, bwd, st);
+  else launch_norm_type<M3D_TYPE_F16>(A, s, grid, bwd, st);
+  M3D_CHECK_LAUNCH();
+  return M3D_OK;
+}
+static bool norm_type_ok(int32_t t) { return t >= M3D_TYPE_F32 && t <= M3D_TYPE_F16; }
+static bool element_aligned(const void* p, int32_t type) { return (((uintptr_t)p) & (type == M3D_TYPE_F32 ? 3 : 1)) == 0; }
+
+extern "C" int m3d_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int64_t rows, int32_t cols, int32_t type,
+                                  int32_t wtype, float eps, float slope, void* y, float* mean, float* rstd, void* stream) {
+  if (rows < 0 || cols < 1 || ldx < 0 || !norm_type_ok(type) || !norm_type_ok(wtype) || !(eps >= 0.f)) return M3D_ERR_INVALID;
+  if (rows == 0) return M3D_OK;
+  if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return M3D_ERR_INVALID;
+  if (!element_aligned(x, type) || !element_aligned(y, type) || !element_aligned(w, wtype) || !element_aligned(b, wtype)) return M3D_ERR_INVALID;
+  NormArgs A{};
+  A.x = x; A.w = w; A.b = b; A.y = y; A.mean = mean; A.rstd = rstd; A.rows = rows; A.ldx = ldx; A.cols = cols; A.wtype = wtype;
+  A.eps = eps; A.slope = slope; A.inv = 1.f / (float)cols;
+  const NormShape s = norm_shape(cols, type);
+  return launch_norm_any(A, s, norm_grid(s, rows), type, false, (hipStream_t)stream);
+}
+
+extern "C" size_t m3d_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t type) {
+  if (rows <= 0 || cols < 1 || !norm_type_ok(type)) return 0;
+  return (size_t)norm_grid(norm_shape(cols, type), rows) * 2 * (size_t)cols * sizeof(float);
+}
+
+extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* b, const float* mean,
+                                  const float* rstd, int64_t rows, int32_t cols, int32_t type, int32_t wtype, float slope, void* dx,
+                                  void* dw, void* db, void* ws, void* stream) {
+  if (rows < 0 || cols < 1 || ldx < 0 || lddy < 0 || !norm_type_ok(type) || !norm_type_ok(wtype)) return M3D_ERR_INVALID;
+  if (rows > 0 && (!dy || !x || !mean || !rstd || ((dw || db) && !ws))) return M3D_ERR_INVALID;
+  if (!element_aligned(x, type) || !element_aligned(dy, type) || !element_aligned(dx, type) || !element_aligned(w, wtype) ||
+      !element_aligned(b, wtype) || !element_aligned(dw, wtype) || !element_aligned(db, wtype) || (((uintptr_t)ws) & 3))
+    return M3D_ERR_INVALID;
+  hipStream_t st = (hipStream_t)stream;
+  NormArgs A{};
+  A.x = x; A.dy = dy; A.w = w; A.b = b; A.dx = dx; A.mean = (float*)mean; A.rstd = (float*)rstd; A.rows = rows; A.ldx = ldx; A.lddy = lddy;
+  A.cols = cols; A.wtype = wtype; A.slope = slope; A.inv = 1.f / (float)cols;
+  A.parts = (dw || db) ? (float*)ws : nullptr;
+  const NormShape s = norm_shape(cols, type);
+  const int64_t grid = norm_grid(s, rows);
+  if (rows > 0 && (dx || A.parts)) {
+    const int rc = launch_norm_any(A, s, grid, type, true, st);
+    if (rc != M3D_OK) return rc;
+  }
+  if (dw || db) {  // (no rows: no parts, zeros)
+    hipLaunchKernelGGL(layer_norm_wgrad_kernel, dim3((unsigned)m3d_cdiv(2 * (int64_t)cols, 16)), dim3(1024), 0, st, (const float*)ws,
+                       (int)grid, cols, wtype, dw, db);
+    M3D_CHECK_LAUNCH();
+  }
+  return M3D_OK;
+}

@@ -1,0 +1,602 @@
+// Optimizer-side kernels over MANY tensors at once (gfx950): the global gradient norm, clipping by it, and the AdamW update with
+// its moments in 32 or in 8 bits.
+//
+//   s = sum g^2,  norm = sqrt(s),  k = min(1, max_norm / (norm + 1e-6)),  g' = k g
+//   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Everything here streams: an element costs a handful of operations and 12 (norm + clip, fp32) to 28 bytes (AdamW, fp32), so the
+// memory bounds all of it and the design is about few launches and few bytes:
+//   * the tensors' pointers travel as KERNEL ARGUMENTS (up to OPT_TENSORS a launch): no table in device memory to upload when a
+//     gradient moves, nothing to keep alive, and a captured graph holds its own copy;
+//   * a tensor is cut into blocks of 256 elements, numbered through over all tensors; a workgroup takes a contiguous run of
+//     blocks and finds its first tensor by a binary search over the arguments (scalar loads).  The moments live in flat buffers in
+//     the same numbering (every tensor's slice starts at a multiple of 256);
+//   * the norm is two steps without a launch of its own in between: workgroups leave fp64 partial sums, and whoever needs the
+//     norm (the clip kernel, the AdamW kernel) adds them up, in a fixed order, at its start;
+//   * vectors are loaded with the alignment of their ELEMENT (unaligned 16-byte accesses are fine on this target), so that views
+//     at odd offsets take the same path.
+#include "m3d_common.h"
+#include "../../include/m3d_hip.h"
+
+#define OPT_TENSORS 152   // 24 bytes each: the list stays under 4 KB of kernel arguments (HipRandLANet has 141 tensors: one launch)
+#define OPT_BLOCK 256     // elements of a block (and of one 8-bit scale)
+#define OPT_PARTS M3D_GRAD_NORM_PARTS
+
+struct TensorList {
+  void* p[OPT_TENSORS];
+  void* g[OPT_TENSORS];             // null: the tensor has no gradient in this step
+  uint32_t blk[OPT_TENSORS + 1];    // number of the tensor's first block
+  uint32_t info[OPT_TENSORS];       // bits 0-7: elements of its last block (0: 256), bits 8-9: type (0 fp32, 1 bf16, 2 fp16)
+  int32_t count, first;             // tensors in the list; number of the first one
+};
+static_assert(sizeof(TensorList) <= 3800, "kernel arguments");
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned short h8u __attribute__((ext_vector_type(8), aligned(2)));
+
+__device__ __forceinline__ float half_bits_to_f32(unsigned short b) { return (float)__builtin_bit_cast(_Float16, b); }
+__device__ __forceinline__ float bits_to_f32(unsigned short b, int type) { return type == 1 ? bf16_to_f32(b) : half_bits_to_f32(b); }
+__device__ __forceinline__ unsigned short f32_to_bits(float v, int type) {
+  return type == 1 ? f32_to_bf16(v) : __builtin_bit_cast(unsigned short, (_Float16)v);
+}
+__device__ __forceinline__ float load1(const void* base, int64_t e, int type) {
+  return type == 0 ? ((const float*)base)[e] : bits_to_f32(((const unsigned short*)base)[e], type);
+}
+__device__ __forceinline__ void store1(void* base, int64_t e, int type, float v) {
+  if (type == 0) ((float*)base)[e] = v;
+  else ((unsigned short*)base)[e] = f32_to_bits(v, type);
+}
+// n (1 .. 4) elements from e on; elements beyond n come back as zeros
+__device__ __forceinline__ void load4(const void* base, int64_t e, int n, int type, float (&v)[4]) {
+  if (n >= 4) {
+    if (type == 0) {
+      const f4u t = *(const f4u*)((const float*)base + e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = t[j];
+    } else {
+      const h4u t = *(const h4u*)((const unsigned short*)base + e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = bits_to_f32(t[j], type);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? load1(base, e + j, type) : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(void* base, int64_t e, int n, int type, const float (&v)[4]) {
+  if (n >= 4) {
+    if (type == 0) {
+      f4u t;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = v[j];
+      *(f4u*)((float*)base + e) = t;
+    } else {
+      h4u t;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = f32_to_bits(v[j], type);
+      *(h4u*)((unsigned short*)base + e) = t;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) store1(base, e + j, type, v[j]);
+  }
+}
+
+// the tensor that block b belongs to (blk[0] <= b < blk[count])
+__device__ __forceinline__ int tensor_of(const TensorList& L, uint32_t b) {
+  int lo = 0, hi = L.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (L.blk[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+__device__ __forceinline__ int64_t tensor_numel(const TensorList& L, int t) {
+  const int last = L.info[t] & 255;
+  return (int64_t)(L.blk[t + 1] - L.blk[t]) * OPT_BLOCK - (last ? OPT_BLOCK - last : 0);
+}
+
+// sum over the 256 threads of a workgroup, the same bits in every thread
+__device__ __forceinline__ double block_sum_d(double v, double* red /* [4] */) {
+  v = wave_sum_d(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+__device__ __forceinline__ double norm_of(const double* __restrict__ parts, int nparts, double* red) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
+  return sqrt(block_sum_d(s, red));
+}
+__device__ __forceinline__ double clip_factor(double norm, double max_norm) {
+  const double k = max_norm / (norm + 1e-6);
+  return k > 1.0 ? 1.0 : k;  // (a NaN norm stays a NaN)
+}
+
+// ---- s: fp64 partial sums of g^2 (the products and sums are exact to 2^-53: the factor that follows, and every 8-bit code
+// behind it, does not depend on how the work was cut).  One workgroup per run of blocks, four 16-byte loads in flight.
+template <int TYPE>
+__device__ __forceinline__ double range_squares(const void* base, int64_t lo, int64_t n) {  // n vectors of 16 bytes from element lo on
+  constexpr int N = TYPE == 0 ? 4 : 8;
+  double s[2] = {0.0, 0.0};
+  auto add = [&](const float (&x)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j & 1] = fma((double)x[j], (double)x[j], s[j & 1]);
+  };
+  auto load = [&](int64_t i, float (&x)[N]) {
+    if constexpr (TYPE == 0) {
+      const f4u t = *(const f4u*)((const float*)base + lo + i * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = t[j];
+    } else {
+      const h8u t = *(const h8u*)((const unsigned short*)base + lo + i * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = bits_to_f32(t[j], TYPE);
+    }
+  };
+  int64_t i = threadIdx.x;
+  for (; i + 3 * 256 < n; i += 4 * 256) {
+    float x[4][N];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load(i + u * 256, x[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add(x[u]);
+  }
+  for (; i < n; i += 256) {
+    float x[N];
+    load(i, x);
+    add(x);
+  }
+  return s[0] + s[1];
+}
+
+__global__ __launch_bounds__(256) void grad_norm_kernel(const TensorList L, uint32_t chunk, double* __restrict__ parts, int add) {
+  __shared__ double red[4];
+  const uint32_t end = L.blk[L.count];
+  double s = 0.0;
+  uint64_t c0 = (uint64_t)L.blk[0] + (uint64_t)blockIdx.x * chunk;
+  if (c0 < end) {
+    const uint32_t c1 = c0 + chunk < end ? (uint32_t)(c0 + chunk) : end;
+    uint32_t b = (uint32_t)c0;
+    for (int t = tensor_of(L, b); b < c1; ++t) {
+      const uint32_t stop = L.blk[t + 1] < c1 ? L.blk[t + 1] : c1;
+      if (L.g[t]) {
+        const int type = (L.info[t] >> 8) & 3;
+        const int64_t lo = (int64_t)(b - L.blk[t]) * OPT_BLOCK;
+        int64_t hi = (int64_t)(stop - L.blk[t]) * OPT_BLOCK;
+        const int64_t all = tensor_numel(L, t);
+        if (hi > all) hi = all;
+        const int64_t per = type == 0 ? 4 : 8, n = (hi - lo) / per, tail = lo + n * per;
+        s += type == 0 ? range_squares<0>(L.g[t], lo, n) : type == 1 ? range_squares<1>(L.g[t], lo, n) : range_squares<2>(L.g[t], lo, n);
+        if (tail + (int64_t)threadIdx.x < hi) {
+          const double x = (double)load1(L.g[t], tail + threadIdx.x, type);
+          s = fma(x, x, s);
+        }
+      }
+      b = stop;
+    }
+  }
+  s = block_sum_d(s, red);
+  if (threadIdx.x == 0) parts[blockIdx.x] = add ? parts[blockIdx.x] + s : s;
+}
+
+// ---- g *= k in place (always written, as the gradients' new values).  The runs are taken in the opposite order of the norm's
+// pass: what that pass read last is still in the 256 MB cache in front of the memory.
+__global__ __launch_bounds__(256) void grad_clip_kernel(const TensorList L, uint32_t chunk, const double* __restrict__ parts, int nparts,
+                                                        double max_norm, float* __restrict__ norm_out) {
+  __shared__ double red[4];
+  const double norm = norm_of(parts, nparts, red);
+  const float k = (float)clip_factor(norm, max_norm);
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  const uint32_t end = L.blk[L.count];
+  const uint64_t c0 = (uint64_t)L.blk[0] + (uint64_t)(gridDim.x - 1 - blockIdx.x) * chunk;
+  if (c0 >= end) return;
+  const uint32_t c1 = c0 + chunk < end ? (uint32_t)(c0 + chunk) : end;
+  uint32_t b = (uint32_t)c0;
+  for (int t = tensor_of(L, b); b < c1; ++t) {
+    const uint32_t stop = L.blk[t + 1] < c1 ? L.blk[t + 1] : c1;
+    if (L.g[t]) {
+      const int type = (L.info[t] >> 8) & 3;
+      int64_t hi = (int64_t)(stop - L.blk[t]) * OPT_BLOCK;
+      const int64_t all = tensor_numel(L, t);
+      if (hi > all) hi = all;
+      for (int64_t e = (int64_t)(b - L.blk[t]) * OPT_BLOCK + threadIdx.x * 4; e < hi; e += 1024) {
+        const int n = hi - e < 4 ? (int)(hi - e) : 4;
+        float v[4];
+        load4(L.g[t], e, n, type, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= k;
+        store4(L.g[t], e, n, type, v);
+      }
+    }
+    b = stop;
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// AdamW.  state (fp32 words): [0] updates done, [1] the master ticket, [2 ..] 64 tickets (uint32, zero between launches); missed[i]:
+// updates that tensor i had no gradient in — its own count is state[0] - missed[i], as torch counts per parameter.
+// ------------------------------------------------------------------------------------------
+struct AdamArgs {
+  void *m, *v;
+  float *ms, *vs;                // block scales (8 bits)
+  float* state;
+  int32_t* missed;
+  const double* parts;           // gradient norm's partial sums, or null: no clipping
+  float* norm_out;
+  const float* lr_dev;           // learning rate on the device, or null
+  double max_norm, lr, log_b1, log_b2, wd;
+  double b1, b2, c1, c2;         // betas and 1 - betas
+  float eps;
+  int32_t nparts, bump;
+  uint32_t chunk;
+};
+
+struct AdamStep { float decay, size, root; };  // p *= decay; p -= size * m / (sqrt(v) * root + eps)
+// 1 - b^t through expm1: at b = 0.999, t = 1 the plain difference in fp32 is off by 1e-5
+__device__ __forceinline__ AdamStep adam_step_of(const AdamArgs& A, double t, double lr) {
+  AdamStep s;
+  s.decay = (float)(1.0 - lr * A.wd);
+  s.size = (float)(lr / -expm1(t * A.log_b1));
+  s.root = (float)(1.0 / sqrt(-expm1(t * A.log_b2)));
+  return s;
+}
+
+// e4m3 (OCP: 4 bits of exponent, 3 of fraction) through the conversion instructions, which round to nearest even; a value comes
+// as a double, and its conversion to 32 bits must not round to a border: the upper word's last bit takes in whether anything is
+// below it, which leaves 16 bits more than the code has.
+__device__ __forceinline__ float sticky_f32(double x) {
+  const int lo = __double2loint(x);
+  return (float)__hiloint2double(__double2hiint(x) | (lo != 0 ? 1 : 0), 0);
+}
+#define NAN_M 0x7fu
+#define NAN_V 0xffu
+#define MIN_SCALE 1.17549435e-38f  // 2^-126
+// decoded, as held: one product in 32 bits
+__device__ __forceinline__ void decode_m4(uint32_t c, float s, float (&m)[4]) {
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  const float k = 0.00390625f;  // 2^-8: the block's largest magnitude is code 256
+  m[0] = a[0] * k * s; m[1] = a[1] * k * s; m[2] = b[0] * k * s; m[3] = b[1] * k * s;
+}
+// u(c) = 2^((c >> 3) - 31) (1 + (c & 7) / 8): the code is the upper part of a float with its exponent moved
+__device__ __forceinline__ float decode_v(uint32_t c, float s) {
+  const float u = __uint_as_float((c << 20) + ((127u - 31u) << 23)) * s;
+  return c == 0u ? 0.f : c == NAN_V ? __builtin_nanf("") : u;
+}
+// what a block's largest finite magnitude is, in every lane of its wave
+__device__ __forceinline__ float wave_max_f(float v) {
+  const int i0 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false);
+  v = fmaxf(v, __int_as_float(i0));
+  const int i1 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false);
+  v = fmaxf(v, __int_as_float(i1));
+  const int i2 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false);
+  v = fmaxf(v, __int_as_float(i2));
+  const int i3 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false);
+  v = fmaxf(v, __int_as_float(i3));
+  return xgroup_max(v, opaque_pinf());
+}
+__device__ __forceinline__ bool finite_f(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// one wave's block of new moments -> codes and scales (every lane: four consecutive elements)
+__device__ __forceinline__ void encode_block(const double (&m)[4], const double (&v)[4], uint32_t& cm, uint32_t& cv, float& sm, float& sv) {
+  float mx = 0.f, vx = 0.f;
+  bool fm[4], fv[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = fabsf((float)m[j]), b = (float)v[j];  // (rounding keeps the order: the largest one's rounding is the scale)
+    fm[j] = finite_f(a); fv[j] = finite_f(b);
+    mx = fmaxf(mx, fm[j] ? a : 0.f);
+    vx = fmaxf(vx, fv[j] ? b : 0.f);
+  }
+  sm = wave_max_f(mx);
+  sv = wave_max_f(vx);
+  if (sm < MIN_SCALE) sm = 0.f;
+  if (sv < MIN_SCALE) sv = 0.f;
+  float r[4];
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    r[j] = fm[j] && sm > 0.f ? sticky_f32(m[j] / (double)sm * 256.0) : 0.f;
+    const double q = sv > 0.f ? v[j] / (double)sv : 0.0;
+    const uint32_t u = __float_as_uint(sticky_f32(q));
+    int k = (int)((u + 0x7ffffu + ((u >> 20) & 1u)) >> 20) - ((127 - 31) << 3);  // nearest even at three bits of fraction
+    k = k < 1 ? 1 : k;                                                            // what is above zero stays above it
+    c[j] = !fv[j] ? NAN_V : q > 0.0 ? (uint32_t)k : 0u;
+  }
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], w, true);
+  cm = (uint32_t)w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) cm = fm[j] ? cm : (cm & ~(0xffu << (8 * j))) | (NAN_M << (8 * j));
+  cv = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
+}
+
+// A workgroup's four waves take the blocks of its run in turn, a lane four consecutive elements (16-byte accesses in fp32).
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const AdamArgs A) {
+  __shared__ double red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const double done = (double)__hip_atomic_load(&A.state[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  double k = 1.0;
+  bool go = true;
+  if (A.parts) {
+    const double norm = norm_of(A.parts, A.nparts, red);
+    k = clip_factor(norm, A.max_norm);
+    go = norm <= 1.7e308;  // a norm that is not finite: the step is not taken (neither counted)
+    if (A.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *A.norm_out = (float)norm;
+  }
+  const uint32_t end = L.blk[L.count];
+  const uint64_t c0 = (uint64_t)L.blk[0] + (uint64_t)(gridDim.x - 1 - blockIdx.x) * A.chunk;  // (against the norm pass's order)
+  if (go && c0 + wave < end) {
+    const double lr = A.lr_dev ? (double)A.lr_dev[0] : A.lr;
+    const float kf = (float)k, b1 = (float)A.b1, b2 = (float)A.b2, d1 = (float)A.c1, d2 = (float)A.c2;
+    const uint32_t c1 = c0 + A.chunk < end ? (uint32_t)(c0 + A.chunk) : end;
+    uint32_t b = __builtin_amdgcn_readfirstlane((uint32_t)c0 + wave);
+    if (b < c1) {
+      int t = tensor_of(L, b), at = -1;
+      AdamStep S{};
+      for (; b < c1; b += 4) {
+        while (b >= L.blk[t + 1]) ++t;
+        void* g = L.g[t];
+        if (!g) {
+          if (b == L.blk[t] && lane == 0) A.missed[L.first + t] += 1;
+          continue;
+        }
+        if (t != at) {
+          S = adam_step_of(A, done + 1.0 - (double)A.missed[L.first + t], lr);
+          at = t;
+        }
+        const int type = (L.info[t] >> 8) & 3, last = L.info[t] & 255;
+        const int64_t e = (int64_t)(b - L.blk[t]) * OPT_BLOCK + lane * 4;
+        int n = (b + 1 == L.blk[t + 1] && last ? last : OPT_BLOCK) - lane * 4;
+        n = n > 4 ? 4 : n;
+        float p[4] = {0.f, 0.f, 0.f, 0.f}, gv[4] = {0.f, 0.f, 0.f, 0.f};
+        const int64_t s = (int64_t)b * 64 + lane;  // the lane's four elements in the flat moments
+        if (n > 0) {
+          load4(g, e, n, type, gv);
+          load4(L.p[t], e, n, type, p);
+        }
+        float mf[4], vf[4];
+        if constexpr (BITS == 32) {
+          const f32x4 m = ((const f32x4*)A.m)[s], v = ((const f32x4*)A.v)[s];
+          f32x4 mo, vo;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = gv[j] * kf;
+            mf[j] = mo[j] = b1 * m[j] + d1 * x;
+            vf[j] = vo[j] = b2 * v[j] + d2 * x * x;
+          }
+          ((f32x4*)A.m)[s] = mo;
+          ((f32x4*)A.v)[s] = vo;
+        } else {
+          const uint32_t qm = ((const uint32_t*)A.m)[s], qv = ((const uint32_t*)A.v)[s];
+          const float sm = A.ms[b], sv = A.vs[b];
+          float om[4];
+          double m[4], v[4];
+          decode_m4(qm, sm, om);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // In 64 bits, every operation rounded by itself: with decimal betas the sums (9 a + b) / 10 hit the borders of 32 bits (the
+            // scale's) one time in ten, and which side they fall to must not depend on what the compiler contracts.
+#pragma clang fp contract(off)
+            const double x = (double)gv[j] * k;
+            m[j] = A.b1 * (double)om[j] + A.c1 * x;
+            v[j] = A.b2 * (double)decode_v((qv >> (8 * j)) & 255u, sv) + A.c2 * (x * x);
+            mf[j] = (float)m[j];
+            vf[j] = (float)v[j];
+          }
+          uint32_t cm, cv;
+          float nm, nv;
+          encode_block(m, v, cm, cv, nm, nv);
+          ((uint32_t*)A.m)[s] = cm;
+          ((uint32_t*)A.v)[s] = cv;
+          if (lane == 0) { A.ms[b] = nm; A.vs[b] = nv; }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = p[j] * S.decay - S.size * mf[j] / (sqrtf(vf[j]) * S.root + A.eps);
+        if (n > 0) store4(L.p[t], e, n, type, p);
+      }
+    }
+  }
+  if (!A.bump) return;
+  __syncthreads();  // every thread of this workgroup has used its copy of the count
+  if (threadIdx.x == 0) {  // two levels of tickets: one address takes ~15 ns an arrival
+    unsigned* tk = (unsigned*)&A.state[1];
+    const unsigned sub = blockIdx.x % 64, members = gridDim.x / 64 + (sub < gridDim.x % 64 ? 1u : 0u);
+    if (atomicAdd(&tk[1 + sub], 1u) == members - 1) {
+      tk[1 + sub] = 0u;
+      const unsigned groups = gridDim.x < 64 ? gridDim.x : 64;
+      if (atomicAdd(&tk[0], 1u) == groups - 1) {
+        if (go) __hip_atomic_store(&A.state[0], (float)(done + 1.0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        tk[0] = 0u;
+      }
+    }
+  }
+}
+
+// ---- 8-bit moments <-> 32 bits (checkpoints, inspection)
+__global__ __launch_bounds__(256) void moments_decode_kernel(const uint32_t* __restrict__ qm, const uint32_t* __restrict__ qv,
+                                                             const float* __restrict__ sm, const float* __restrict__ sv,
+                                                             f32x4* __restrict__ m, f32x4* __restrict__ v, int64_t n4) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+    float a[4];
+    decode_m4(qm[i], sm[i >> 6], a);
+    const uint32_t c = qv[i];
+    const float s = sv[i >> 6];
+    m[i] = f32x4{a[0], a[1], a[2], a[3]};
+    v[i] = f32x4{decode_v(c & 255u, s), decode_v((c >> 8) & 255u, s), decode_v((c >> 16) & 255u, s), decode_v(c >> 24, s)};
+  }
+}
+__global__ __launch_bounds__(256) void moments_encode_kernel(const f32x4* __restrict__ m, const f32x4* __restrict__ v,
+                                                             uint32_t* __restrict__ qm, uint32_t* __restrict__ qv,
+                                                             float* __restrict__ sm, float* __restrict__ sv, int64_t blocks) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); b < blocks; b += (int64_t)gridDim.x * 4) {
+    const f32x4 a = m[b * 64 + lane], c = v[b * 64 + lane];
+    const double md[4] = {a[0], a[1], a[2], a[3]}, vd[4] = {c[0], c[1], c[2], c[3]};
+    uint32_t cm, cv;
+    float nm, nv;
+    encode_block(md, vd, cm, cv, nm, nv);
+    qm[b * 64 + lane] = cm;
+    qv[b * 64 + lane] = cv;
+    if (lane == 0) { sm[b] = nm; sv[b] = nv; }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+static int check_tensors(void* const* ptrs, const int64_t* numel, const int32_t* types, int32_t count, int64_t* blocks) {
+  if (count < 0 || (count > 0 && (!ptrs || !numel || !types)) ) return M3D_ERR_INVALID;
+  int64_t b = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (numel[i] < 0 || types[i] < 0 || types[i] > 2) return M3D_ERR_INVALID;
+    if (((uintptr_t)ptrs[i]) & (types[i] == 0 ? 3 : 1)) return M3D_ERR_INVALID;
+    if (numel[i] > ((int64_t)1 << 39)) return M3D_ERR_UNSUPPORTED;
+    b += m3d_cdiv(numel[i], OPT_BLOCK);
+    if (b > 0xfffffff0ll) return M3D_ERR_UNSUPPORTED;  // (blocks are numbered in 32 bits)
+  }
+  *blocks = b;
+  return M3D_OK;
+}
+// the tensors from `from` on that fit one launch (tensors without elements take no blocks and stay out of the search); the next one
+static int32_t fill_list(TensorList& L, void* const* params, void* const* grads, const int64_t* numel, const int32_t* types, int32_t from,
+                         int32_t count, uint32_t block) {
+  int32_t n = 0, i = from;
+  L.first = from;
+  for (; i < count && n < OPT_TENSORS; ++i, ++n) {
+    L.p[n] = params ? params[i] : nullptr;
+    L.g[n] = grads[i];
+    L.blk[n] = block;
+    L.info[n] = (uint32_t)((numel[i] & 255) | ((int64_t)types[i] << 8));
+    block += (uint32_t)m3d_cdiv(numel[i], OPT_BLOCK);
+  }
+  L.blk[n] = block;
+  L.count = n;
+  return i;
+}
+// blocks a workgroup takes, so that at most `most` workgroups run
+static uint32_t chunk_of(int64_t blocks, int64_t least, int64_t most) {
+  const int64_t c = m3d_cdiv(blocks, most);
+  return (uint32_t)(c < least ? least : c);
+}
+
+extern "C" int m3d_grad_norm(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count, double* parts, int32_t* nparts,
+                             void* stream) {
+  int64_t blocks = 0;
+  const int rc = check_tensors(grads, numel, types, count, &blocks);
+  if (rc != M3D_OK) return rc;
+  if (!parts || !nparts) return M3D_ERR_INVALID;
+  TensorList L;
+  // the first launch leaves a value in every part
+  uint32_t grid = 1;
+  for (int32_t i = 0; i < count;) {
+    i = fill_list(L, nullptr, grads, numel, types, i, count, 0);
+    const int64_t n = L.blk[L.count], w = m3d_cdiv(n, chunk_of(n, 1, OPT_PARTS));
+    if (w > grid) grid = (uint32_t)w;
+  }
+  int32_t i = 0, add = 0;
+  do {
+    i = count ? fill_list(L, nullptr, grads, numel, types, i, count, 0) : 0;
+    if (!count) { L.count = 0; L.blk[0] = 0; L.first = 0; }
+    const int64_t n = L.blk[L.count];
+    const uint32_t chunk = chunk_of(n, 1, OPT_PARTS);
+    const uint32_t gx = add ? (uint32_t)m3d_cdiv(n, chunk) : grid;
+    if (gx > 0) hipLaunchKernelGGL(grad_norm_kernel, dim3(gx), dim3(256), 0, (hipStream_t)stream, L, chunk, parts, add);
+    M3D_CHECK_LAUNCH();
+    add = 1;
+  } while (i < count);
+  *nparts = (int32_t)grid;
+  return M3D_OK;
+}
+
+extern "C" int m3d_clip_grads(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count, const double* parts,
+                              int32_t nparts, double max_norm, float* norm_out, void* stream) {
+  int64_t blocks = 0;
+  const int rc = check_tensors(grads, numel, types, count, &blocks);
+  if (rc != M3D_OK) return rc;
+  if (!parts || nparts < 1 || nparts > OPT_PARTS || !(max_norm >= 0.0)) return M3D_ERR_INVALID;
+  TensorList L;
+  for (int32_t lists = (int32_t)m3d_cdiv(count, OPT_TENSORS), l = lists > 0 ? lists - 1 : 0; l >= 0; --l) {  // (last list first, see the kernel)
+    if (count) fill_list(L, nullptr, grads, numel, types, l * OPT_TENSORS, count, 0);
+    else { L.count = 0; L.blk[0] = 0; L.first = 0; }
+    const int64_t n = L.blk[L.count];
+    const uint32_t chunk = chunk_of(n, 1, 2048);
+    const int64_t gx = m3d_cdiv(n, chunk);
+    if (gx == 0 && l > 0) continue;  // (the last launch writes the norm)
+    hipLaunchKernelGGL(grad_clip_kernel, dim3((unsigned)(gx > 0 ? gx : 1)), dim3(256), 0, (hipStream_t)stream, L, chunk, parts, nparts, max_norm,
+                       l == 0 ? norm_out : nullptr);
+    M3D_CHECK_LAUNCH();
+  }
+  return M3D_OK;
+}
+
+extern "C" int m3d_adamw_step(const M3DAdamW* a, void* stream) {
+  if (!a) return M3D_ERR_INVALID;
+  int64_t blocks = 0, same = 0;
+  int rc = check_tensors(a->params, a->numel, a->types, a->count, &blocks);
+  if (rc == M3D_OK) rc = check_tensors(a->grads, a->numel, a->types, a->count, &same);
+  if (rc != M3D_OK) return rc;
+  if (!a->state || (a->count > 0 && !a->missed)) return M3D_ERR_INVALID;
+  if (a->state_bits != 32 && a->state_bits != 8) return M3D_ERR_UNSUPPORTED;
+  if (blocks > 0 && (!a->exp_avg || !a->exp_avg_sq || (a->state_bits == 8 && (!a->scale_avg || !a->scale_avg_sq)))) return M3D_ERR_INVALID;
+  if ((((uintptr_t)a->exp_avg) | ((uintptr_t)a->exp_avg_sq)) & 15) return M3D_ERR_INVALID;
+  for (int32_t i = 0; i < a->count; ++i)
+    if (a->numel[i] > 0 && !a->params[i]) return M3D_ERR_INVALID;
+  if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return M3D_ERR_INVALID;
+  if (a->parts && (a->nparts < 1 || a->nparts > OPT_PARTS || !(a->max_norm >= 0.0))) return M3D_ERR_INVALID;
+  AdamArgs A{};
+  A.m = a->exp_avg; A.v = a->exp_avg_sq; A.ms = a->scale_avg; A.vs = a->scale_avg_sq;
+  A.state = a->state; A.missed = a->missed; A.parts = a->parts; A.nparts = a->nparts; A.lr_dev = a->lr_dev;
+  A.max_norm = a->max_norm; A.lr = a->lr; A.wd = a->weight_decay; A.eps = (float)a->eps;
+  A.b1 = a->beta1; A.b2 = a->beta2; A.c1 = 1.0 - a->beta1; A.c2 = 1.0 - a->beta2;
+  A.log_b1 = log(a->beta1); A.log_b2 = log(a->beta2);
+  TensorList L;
+  const int32_t lists = (int32_t)m3d_cdiv(a->count > 0 ? a->count : 1, OPT_TENSORS);
+  for (int32_t l = lists - 1; l >= 0; --l) {  // (last list first: against the order of the norm's pass)
+    uint32_t start = 0;
+    for (int32_t i = 0; i < l * OPT_TENSORS; ++i) start += (uint32_t)m3d_cdiv(a->numel[i], OPT_BLOCK);
+    if (a->count) fill_list(L, a->params, a->grads, a->numel, a->types, l * OPT_TENSORS, a->count, start);
+    else { L.count = 0; L.blk[0] = 0; L.first = 0; }
+    const int64_t n = (int64_t)L.blk[L.count] - L.blk[0];
+    A.chunk = chunk_of(n, 4, 2048);
+    A.bump = l == 0;
+    A.norm_out = l == 0 ? a->norm_out : nullptr;
+    const int64_t gx = m3d_cdiv(n, A.chunk);
+    if (gx == 0 && l > 0) continue;
+    const dim3 grid((unsigned)(gx > 0 ? gx : 1));  // (the last launch counts the step)
+    if (a->state_bits == 32) hipLaunchKernelGGL(adamw_kernel<32>, grid, dim3(256), 0, (hipStream_t)stream, L, A);
+    else hipLaunchKernelGGL(adamw_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, L, A);
+    M3D_CHECK_LAUNCH();
+  }
+  return M3D_OK;
+}
+
+extern "C" int m3d_moments_decode(const void* exp_avg, const void* exp_avg_sq, const float* scale_avg, const float* scale_avg_sq,
+                                  float* avg_out, float* avg_sq_out, int64_t blocks, void* stream) {
+  if (blocks < 0) return M3D_ERR_INVALID;
+  if (blocks == 0) return M3D_OK;
+  if (!exp_avg || !exp_avg_sq || !scale_avg || !scale_avg_sq || !avg_out || !avg_sq_out) return M3D_ERR_INVALID;
+  if ((((uintptr_t)exp_avg) | ((uintptr_t)exp_avg_sq)) & 3 || (((uintptr_t)avg_out) | ((uintptr_t)avg_sq_out)) & 15) return M3D_ERR_INVALID;
+  int64_t gx = m3d_cdiv(blocks * 64, 256);
+  if (gx > 8192) gx = 8192;
+  hipLaunchKernelGGL(moments_decode_kernel, dim3((unsigned)gx), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)exp_avg,
+                     (const uint32_t*)exp_avg_sq, scale_avg, scale_avg_sq, (f32x4*)avg_out, (f32x4*)avg_sq_out, blocks * 64);
+  M3D_CHECK_LAUNCH();
+  return M3D_OK;
+}
+extern "C" int m3d_moments_encode(const float* avg, const float* avg_sq, void* exp_avg, void* exp_avg_sq, float* scale_avg,
+                                  float* scale_avg_sq, int64_t blocks, void* stream) {
+  if (blocks < 0) return M3D_ERR_INVALID;
+  if (blocks == 0) return M3D_OK;
+  if (!exp_avg || !exp_avg_sq || !scale_avg || !scale_avg_sq || !avg || !avg_sq) return M3D_ERR_INVALID;
+  if ((((uintptr_t)exp_avg) | ((uintptr_t)exp_avg_sq)) & 3 || (((uintptr_t)avg) | ((uintptr_t)avg_sq)) & 15) return M3D_ERR_INVALID;
+  int64_t gx = m3d_cdiv(blocks, 4);
+  if (gx > 4096) gx = 4096;
+  hipLaunchKernelGGL(moments_encode_kernel, dim3((unsigned)gx), dim3(256), 0, (hipStream_t)stream, (const f32x4*)avg, (const f32x4*)avg_sq,
+                     (uint32_t*)exp_avg, (uint32_t*)exp_avg_sq, scale_avg, scale_avg_sq, blocks);
+  M3D_CHECK_LAUNCH();
+  return M3D_OK;
+}

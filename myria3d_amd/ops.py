@@ -6,6 +6,7 @@ device memory, to provide the stream and for autograd bookkeeping.  Reference ca
 """
 from __future__ import annotations
 
+import contextlib
 import os
 from typing import List, Optional, Tuple
 
@@ -33,6 +34,14 @@ def _st():
     if _raw_stream is not None:
         return _raw_stream(_cur_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Guard for a launch on ``dev``'s current stream; nothing where ``dev`` is the current device already."""
+    return _NO_GUARD if _cur_device is not None and dev.index == _cur_device() else torch.cuda.device(dev)
 
 
 def capture_id(stream) -> int:
@@ -1621,6 +1630,96 @@ def idw_interpolate(x: Tensor, idx: Tensor, d2: Tensor) -> Tensor:
     y = torch.empty((nq, x.shape[1]), dtype=torch.float32, device=x.device)
     call("m3d_idw_interpolate_fwd", _p(_chk(x)), x.stride(0), _p(idx), _p(d2), nq, k, x.shape[1], _p(y), _st())
     return y
+
+
+# --------------------------------------------------------------------------------------------------
+# layer norm (a SharedMLP's normalisation where batch statistics are none: norm="layer" of HipPointNet2)
+# --------------------------------------------------------------------------------------------------
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # M3D_TYPE_* of include/m3d_hip.h
+
+
+def _rows_of(t: Tensor) -> Tensor:
+    """``t`` as ``[rows, cols]`` with elements of a row next to each other: a view where its strides allow one."""
+    cols = t.shape[-1]
+    t = t.view(-1, cols) if t.is_contiguous() else t.reshape(-1, cols)
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+
+
+def _layer_norm_fwd(rows: Tensor, shape, w: Optional[Tensor], b: Optional[Tensor], wtype: int, eps: float, slope: float, stats: bool):
+    n, cols = rows.shape
+    dev = rows.device
+    y = torch.empty(shape, dtype=rows.dtype, device=dev)
+    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=dev).unbind(0) if stats else (None, None)
+    with on_device(dev):
+        call("m3d_layer_norm_fwd", rows.data_ptr(), rows.stride(0), _p(w), _p(b), n, cols, TYPES[rows.dtype], wtype, eps, slope,
+             y.data_ptr(), _p(mean), _p(rstd), _st())
+    return y, mean, rstd
+
+
+class LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, wtype, eps, slope):
+        rows = _rows_of(x)
+        y, mean, rstd = _layer_norm_fwd(rows, x.shape, w, b, wtype, eps, slope, True)
+        ctx.save_for_backward(rows, w, b, mean, rstd)
+        ctx.args = (x.shape, wtype, slope)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        rows, w, b, mean, rstd = ctx.saved_tensors
+        shape, wtype, slope = ctx.args
+        n, cols = rows.shape
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dy = _rows_of(dy)
+        dx = torch.empty(shape, dtype=rows.dtype, device=rows.device) if need_x else None
+        dw = torch.empty_like(w) if need_w else None
+        db = torch.empty_like(b) if need_b else None
+        ws = None
+        if need_w or need_b:
+            ws = torch.empty(lib().m3d_layer_norm_bwd_workspace_bytes(n, cols, TYPES[rows.dtype]), dtype=torch.uint8, device=rows.device)
+        with on_device(rows.device):
+            call("m3d_layer_norm_bwd", dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), _p(w), _p(b), _p(mean), _p(rstd), n,
+                 cols, TYPES[rows.dtype], wtype, slope, _p(dx), _p(dw), _p(db), _p(ws), _st())
+        return dx, dw, db, None, None, None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
+               negative_slope: Optional[float] = None) -> Tensor:
+    """``torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)``, differentiable (once) in ``x``, ``weight`` and
+    ``bias``; with ``negative_slope`` the LeakyReLU that follows it, in the same pass over the data.
+
+    ``x``: fp32, bf16 or fp16, any shape whose last dimension is not empty; rows may have a stride of their own (a slice of a wider
+    matrix is read in place, an order with other than the last dimension innermost is copied).  ``weight`` / ``bias``: contiguous,
+    of one of these types, both of the same — fp32 parameters over bf16 activations are fine.  Statistics, sums and gradients
+    are held in 32 bits or more; the result has ``x``'s type, the gradients their tensor's.  Same inputs, same bits."""
+    if x.dtype not in TYPES:
+        raise TypeError(f"layer_norm: x must be float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: x needs a last dimension of one element at least, got shape {tuple(x.shape)}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.dtype not in TYPES or t.device != x.device:
+            raise TypeError(f"layer_norm: {name} must be float32, bfloat16 or float16 on {x.device}, got {t.dtype} on {t.device}")
+        if t.shape != x.shape[-1:] or not t.is_contiguous():
+            raise ValueError(f"layer_norm: {name} must be a contiguous vector of {x.shape[-1]} elements, got shape {tuple(t.shape)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"layer_norm: weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
+    if not eps >= 0.0:
+        raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
+    slope = 1.0 if negative_slope is None else float(negative_slope)
+    if not slope >= 0.0:
+        # (the backward pass finds the activation's side from the sign of its argument: any slope would do but a NaN)
+        raise ValueError(f"layer_norm: negative_slope must not be negative, got {negative_slope}")
+    if not x.is_cuda:
+        raise RuntimeError("layer_norm runs on an MI355X only (no CPU fallback by design)")
+    wtype = TYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype]
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return LayerNormFn.apply(x, weight, bias, wtype, float(eps), slope)
+    return _layer_norm_fwd(_rows_of(x), x.shape, weight, bias, wtype, float(eps), slope, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------

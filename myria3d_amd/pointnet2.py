@@ -88,8 +88,10 @@ class HipPointNet2(nn.Module):
     """
 
     def __init__(self, num_features: int, num_classes: int, decimation: int = 4, num_neighbors: int = 32,
-                 return_logits: bool = False, subsampling: str = "fps", random_start: bool = False):
+                 return_logits: bool = False, subsampling: str = "fps", random_start: bool = False, norm: str = "batch"):
         super().__init__()
+        if norm not in ("batch", "layer"):
+            raise ValueError(f"norm must be 'batch' or 'layer', got {norm!r}")
         if subsampling not in ("fps", "random"):
             raise ValueError(f"subsampling must be 'fps' or 'random', got {subsampling!r}")
         if not 1 <= num_neighbors <= 64:
@@ -98,16 +100,18 @@ class HipPointNet2(nn.Module):
         self.decimation, self.num_neighbors, self.return_logits = decimation, num_neighbors, return_logits
         self.subsampling, self.random_start = subsampling, random_start
         self.matmul_precision = "fp32"
+        self.norm = norm
+        ln = norm == "layer"
         c = num_features
         sas = []
         for widths in SA_WIDTHS:
-            sas.append(SAParams(SharedMLPParams([c + 3, *widths])))
+            sas.append(SAParams(SharedMLPParams([c + 3, *widths], layer_norm=ln)))
             c = widths[-1]
         self.sa1, self.sa2, self.sa3 = sas
-        self.fp3 = FPParams(SharedMLPParams([256 + 128, 128]))
-        self.fp2 = FPParams(SharedMLPParams([128 + 64, 64]))
-        self.fp1 = FPParams(SharedMLPParams([64 + num_features, 64]))
-        self.mlp_classif = SharedMLPParams([64, 64, 32], dropout=[0.0, 0.5])
+        self.fp3 = FPParams(SharedMLPParams([256 + 128, 128], layer_norm=ln))
+        self.fp2 = FPParams(SharedMLPParams([128 + 64, 64], layer_norm=ln))
+        self.fp1 = FPParams(SharedMLPParams([64 + num_features, 64], layer_norm=ln))
+        self.mlp_classif = SharedMLPParams([64, 64, 32], dropout=[0.0, 0.5], layer_norm=ln)
         self.fc_classif = nn.Linear(32, num_classes)
         self._plans: Dict[tuple, SAPlan] = {}
         self.last_sample_idx: List[Tensor] = []
@@ -136,6 +140,14 @@ class HipPointNet2(nn.Module):
     def _layer(self, mlp: SharedMLPParams, li: int, x0: Tensor, x1: Optional[Tensor], rows: Optional[Tensor], w: Tensor,
                train: bool, grad_eval: bool) -> Tensor:
         lin, bn = mlp.lins[li], mlp.norms[li].module
+        if self.norm == "layer":
+            x = x0 if rows is None else ops.GatherRowsFn.apply(x0, rows)
+            x = x if x1 is None else torch.cat([x, x1], dim=1)
+            if train or grad_eval:
+                z = ops.LinearFn.apply(x, w, lin.bias)
+            else:
+                z = ops.gemm(x, w, x.shape[0], w.shape[0], x.shape[1], bias=lin.bias)
+            return ops.layer_norm(z, bn.weight, bn.bias, bn.eps, ops.LRELU_SLOPE if mlp.act else None)
         if train:
             return ops.SharedLayerTrainFn.apply(x0, x1, w, lin.bias, bn.weight, bn.bias, bn, mlp.act, rows, None,
                                                 self._bf16, None, None)
@@ -262,6 +274,8 @@ class HipPointNet2(nn.Module):
             raise ValueError(f"expected {self.num_features} features per point, got {x.shape[1]}")
         if self.matmul_precision not in ("fp32", "bf16"):
             raise ValueError(f"matmul_precision must be 'fp32' or 'bf16', got {self.matmul_precision!r}")
+        if self.norm == "layer" and self.matmul_precision != "fp32":
+            raise ValueError("norm='layer' runs in fp32 only")
         self._bf16 = self.matmul_precision == "bf16"
         train = self.training
         grad_eval = (not train) and torch.is_grad_enabled() and (

@@ -28,17 +28,25 @@ class _BatchNormHolder(nn.Module):
         self.module = nn.BatchNorm1d(channels, eps=ops.BN_EPS, momentum=ops.BN_MOMENTUM)
 
 
+class _LayerNormHolder(nn.Module):
+    def __init__(self, channels: int):
+        super().__init__()
+        self.module = nn.LayerNorm(channels)
+
+
 class SharedMLPParams(nn.Module):
-    """Parameters of ``SharedMLP(channels, ...)`` (pyg_randla_net.py:97-109)."""
+    """Parameters of ``SharedMLP(channels, ...)`` (pyg_randla_net.py:97-109).  ``layer_norm``: every point's channels are
+    normalised by themselves (PyG MLP's ``norm="layer_norm"``) instead of every channel over the batch."""
 
     def __init__(self, channels: Sequence[int], act: bool = True, norm: bool = True, bias: bool = True,
-                 dropout: Optional[Sequence[float]] = None):
+                 dropout: Optional[Sequence[float]] = None, layer_norm: bool = False):
         super().__init__()
         nl = len(channels) - 1
         self.act, self.has_norm = act, norm
         self.dropout = list(dropout) if dropout is not None else [0.0] * nl
         self.lins = nn.ModuleList([nn.Linear(channels[i], channels[i + 1], bias=bias) for i in range(nl)])
-        self.norms = nn.ModuleList([_BatchNormHolder(channels[i + 1]) if norm else nn.Identity() for i in range(nl)])
+        holder = _LayerNormHolder if layer_norm else _BatchNormHolder
+        self.norms = nn.ModuleList([holder(channels[i + 1]) if norm else nn.Identity() for i in range(nl)])
 
 
 class LFAParams(nn.Module):

@@ -5,15 +5,22 @@
 * ``FusedAdam`` — ``torch.optim.Adam`` (``/root/reference/configs/model/optimizer/Adam.yaml:1-4``) as ONE kernel
   launch over the flat parameter / gradient buffers of a ``HipRandLANet`` that has run ``flatten_parameters()``;
   stock torch runs ~250 small launches for the same update (141 parameter tensors).
+* ``AdamW`` — ``torch.optim.AdamW`` over any list of parameter tensors (a net that is not flattened, ``HipPointNet2``, frozen
+  parts, several groups, bf16 or fp16 parameters), 152 tensors a launch, its moments in 32 or in 8 bits, clipping included.
+* ``clip_grad_norm_`` — ``torch.nn.utils.clip_grad_norm_`` (Lightning's ``gradient_clip_val``) in two passes over all gradients.
 """
 from __future__ import annotations
 
-from typing import Optional
+import ctypes
+import math
+from array import array
+from typing import Dict, Iterable, List, Optional, Tuple, Union
 
 import torch
 import torch.distributed as dist
+from torch import Tensor
 
-from . import ops
+from . import _lib, ops
 from ._lib import call
 from .ops import cross_entropy  # noqa: F401  (re-export)
 
@@ -157,3 +164,327 @@ class FusedAdam(torch.optim.Optimizer):
 
     def zero_grad(self, set_to_none: bool = False):  # gradients are views of the flat buffer: never detach them
         self.net.flat_grads.zero_()
+
+
+# --------------------------------------------------------------------------------------------------
+# many tensors at once
+# --------------------------------------------------------------------------------------------------
+BLOCK = 256  # elements of a block of the flat moments (every tensor's slice starts at a multiple of it)
+GRAD_NORM_PARTS = 1024  # M3D_GRAD_NORM_PARTS
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether the elements of ``t`` fill one run of memory, in whatever order of dimensions."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: (d[1], d[0])):
+        if size == 1:
+            continue
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _like(g: Tensor, p: Tensor) -> Tensor:
+    """``g`` in the memory order of ``p`` (itself where it has that already)."""
+    if g.stride() == p.stride() or (g.is_contiguous() and p.is_contiguous()):
+        return g
+    return torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+
+
+def _check_grad(g: Tensor) -> None:
+    if g.is_sparse or g.layout is not torch.strided:
+        raise RuntimeError("sparse gradients are not supported")
+
+
+class _Pointers:
+    """The host arrays that the entry points read (pointers, sizes, types of a list of tensors)."""
+
+    def __init__(self, numel: Iterable[int], types: Iterable[int]):
+        self.numel, self.types = array("q", numel), array("i", types)
+        self.count = len(self.numel)
+        self.args = (self.numel.buffer_info()[0], self.types.buffer_info()[0], self.count)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float) -> Tensor:
+    """``torch.nn.utils.clip_grad_norm_(parameters, max_norm)`` for the 2-norm: scales all gradients in place by
+    ``min(1, max_norm / (norm + 1e-6))`` and returns the norm they had together, a 0-dim fp32 tensor on their device (nothing is
+    read back).  fp32, bf16 and fp16 gradients, mixed as they come, on one device; parameters without one are left out.  The norm
+    is summed in 64 bits in a fixed order: the same gradients give the same bits.  Gradients that are not finite scale as in
+    torch (an infinite norm: zeros, NaN for the infinite ones themselves; a NaN norm: NaN)."""
+    params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
+    grads = [p.grad for p in params]
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device=params[0].device if params else "cpu")
+    dev = grads[0].device
+    types = ops.TYPES
+    seen = set()
+    for g in grads:
+        _check_grad(g)
+        if g.device != dev:
+            raise ValueError(f"clip_grad_norm_: all gradients must be on one device, got {dev} and {g.device}")
+        if g.dtype not in types:
+            raise TypeError(f"clip_grad_norm_: gradients must be float32, bfloat16 or float16, got {g.dtype}")
+        if id(g) in seen:
+            raise ValueError("clip_grad_norm_: the same gradient twice")
+        seen.add(id(g))
+    if dev.type != "cuda":
+        raise RuntimeError("clip_grad_norm_ runs on an MI355X only (no CPU fallback by design)")
+    dense = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
+    at = _Pointers([g.numel() for g in dense], [types[g.dtype] for g in dense])
+    ptrs = array("Q", [g.data_ptr() for g in dense])
+    parts = torch.empty(GRAD_NORM_PARTS, dtype=torch.float64, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nparts = ctypes.c_int32(0)
+    with ops.on_device(dev):
+        st = ops._st()
+        call("m3d_grad_norm", ptrs.buffer_info()[0], *at.args, parts.data_ptr(), ctypes.addressof(nparts), st)
+        call("m3d_clip_grads", ptrs.buffer_info()[0], *at.args, parts.data_ptr(), nparts.value, max_norm, norm.data_ptr(), st)
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+class _Group:
+    """What one parameter group of ``AdamW`` keeps: sizes and types of its tensors, its moments (flat, in blocks of 256), counters."""
+
+    def __init__(self, params: List[Tensor], bits: int):
+        self.params, self.bits = params, bits
+        self.at = _Pointers([p.numel() for p in params], [ops.TYPES[p.dtype] for p in params])
+        self.starts, blocks = [], 0
+        for p in params:
+            self.starts.append(blocks * BLOCK)
+            blocks += -(-p.numel() // BLOCK)
+        self.blocks = blocks
+        dev = params[0].device
+        self.avg, self.avg_sq = (torch.zeros(blocks * BLOCK, dtype=torch.float32 if bits == 32 else torch.uint8, device=dev) for _ in range(2))
+        self.scale = self.scale_sq = None
+        if bits == 8:
+            self.scale, self.scale_sq = (torch.zeros(blocks, dtype=torch.float32, device=dev) for _ in range(2))
+        self.state = torch.zeros(66, dtype=torch.float32, device=dev)  # (M3D_ADAM_STATE_WORDS)
+        self.missed = torch.zeros(len(params), dtype=torch.int32, device=dev)
+
+    def slice(self, flat: Tensor, i: int) -> Tensor:
+        """Tensor ``i``'s part of a flat buffer, in its shape and memory order."""
+        p = self.params[i]
+        return flat[self.starts[i]:self.starts[i] + p.numel()].as_strided(p.shape, p.stride(), flat.storage_offset() + self.starts[i])
+
+    def blocks_of(self, scale: Tensor, i: int) -> Tensor:
+        a = self.starts[i] // BLOCK
+        return scale[a:a + -(-self.params[i].numel() // BLOCK)]
+
+    def decoded(self) -> Tuple[Tensor, Tensor]:
+        if self.bits == 32:
+            return self.avg, self.avg_sq
+        m, v = torch.empty((2, self.blocks * BLOCK), dtype=torch.float32, device=self.avg.device).unbind(0)
+        with ops.on_device(self.avg.device):
+            call("m3d_moments_decode", self.avg.data_ptr(), self.avg_sq.data_ptr(), self.scale.data_ptr(), self.scale_sq.data_ptr(),
+                 m.data_ptr(), v.data_ptr(), self.blocks, ops._st())
+        return m, v
+
+    def encode(self, m: Tensor, v: Tensor) -> None:
+        with ops.on_device(self.avg.device):
+            call("m3d_moments_encode", m.data_ptr(), v.data_ptr(), self.avg.data_ptr(), self.avg_sq.data_ptr(), self.scale.data_ptr(),
+                 self.scale_sq.data_ptr(), self.blocks, ops._st())
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` (``amsgrad=False``, ``maximize=False``; with ``weight_decay=0`` also ``torch.optim.Adam``, the
+    reference's optimizer) over any parameter tensors on one device: one launch updates up to 152 of them, one more in front of it
+    where gradients are clipped.  fp32, bf16 and fp16 parameters, mixed as they come; the update is computed in 32 bits and rounded
+    once to the parameter's type.  A parameter without a gradient is left out of a step and keeps its own count, as in torch.
+
+    ``state_bits=8`` holds both moments in a byte an element (with one fp32 scale per 256 elements and moment): 2.03 instead of
+    8 bytes an element.  ``exp_avg`` keeps 4 bits of exponent and 3 of fraction of its block's largest magnitude, ``exp_avg_sq`` 5
+    and 3, so that an element may be 2^-17 of its block's largest gradient before it is lost; a positive second moment never
+    becomes zero.  A value that is not finite is held as NaN, in its own element only.
+
+    ``max_grad_norm``: the gradients of ALL parameters are taken as ``clip_grad_norm_`` would leave them (``p.grad`` itself is
+    not written); ``grad_norm`` is then the norm they had, a 0-dim fp32 tensor on the device.  A step whose norm is not finite
+    changes nothing and is not counted.
+
+    ``lr`` may be a 0-dim fp32 tensor on the device (a schedule under graph replay).  Nothing is read back and step counts live on the
+    device: ``step()`` may be captured into a hipGraph (after one eager step) and replayed; the gradients must then be written in
+    place.  ``state_dict()`` has torch's layout (``step``, ``exp_avg``, ``exp_avg_sq`` per parameter), and with 32 bits states travel
+    to and from ``torch.optim.AdamW`` / ``Adam``; with 8 bits the codes and scales are stored, and 32-bit states are taken in too."""
+
+    def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32, max_grad_norm: Optional[float] = None):
+        if state_bits not in (32, 8):
+            raise ValueError(f"AdamW: state_bits must be 32 or 8, got {state_bits}")
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError(f"AdamW: max_grad_norm must not be negative, got {max_grad_norm}")
+        self.state_bits, self.max_grad_norm = state_bits, None if max_grad_norm is None else float(max_grad_norm)
+        self._groups: List[_Group] = []
+        self._device = None
+        self.grad_norm: Optional[Tensor] = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        if self.max_grad_norm is not None:
+            self.grad_norm = torch.zeros((), dtype=torch.float32, device=self._device)
+            self._parts = torch.empty(GRAD_NORM_PARTS, dtype=torch.float64, device=self._device)
+
+    @staticmethod
+    def _check_group(g: dict, bits: int) -> None:
+        lr, (b1, b2), eps, wd = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+        if isinstance(lr, Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError("AdamW: a tensor lr must be one fp32 element on the device")
+        elif not (float(lr) >= 0.0 and math.isfinite(lr)):
+            raise ValueError(f"AdamW: lr must not be negative, got {lr}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1), got {(b1, b2)}")
+        if not (eps >= 0.0 and wd >= 0.0):
+            raise ValueError(f"AdamW: eps and weight_decay must not be negative, got {eps} and {wd}")
+        if bits == 8 and not eps > 0.0:
+            raise ValueError("AdamW: state_bits=8 needs eps > 0 (a second moment may be held as zero)")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            params = group["params"]
+            if not params:
+                raise ValueError("AdamW: a parameter group without parameters")
+            self._check_group(group, self.state_bits)
+            if len({id(p) for p in params}) < len(params):
+                raise ValueError("AdamW: the same parameter twice in a group")
+            dev = self._device or params[0].device
+            for p in params:
+                if p.dtype not in ops.TYPES:
+                    raise TypeError(f"AdamW: parameters must be float32, bfloat16 or float16, got {p.dtype}")
+                if not _dense(p):
+                    raise ValueError(f"AdamW: a parameter's elements must fill one run of memory, got strides {p.stride()} for {tuple(p.shape)}")
+                if p.device != dev or p.device.type != "cuda":
+                    raise RuntimeError(f"AdamW: all parameters must be on one MI355X (no CPU fallback by design), got {p.device} and {dev}")
+        except Exception:
+            self.param_groups.pop()
+            raise
+        self._device = dev
+        self._groups.append(_Group(list(params), self.state_bits))
+
+    # ------------------------------------------------------------------------------------------
+    def _gradients(self, k: int, group: dict) -> Tuple[array, List[Tensor]]:
+        """Pointers of a group's gradients (0: none) and the tensors to keep alive until they have been read."""
+        out, keep = array("Q"), []
+        for p in group["params"]:
+            g = p.grad
+            if g is None:
+                out.append(0)
+                continue
+            if g.dtype != p.dtype:
+                raise TypeError(f"AdamW: a gradient must have its parameter's type, got {g.dtype} for {p.dtype}")
+            if not (g.is_contiguous() and p.is_contiguous()):
+                _check_grad(g)
+                g = _like(g, p)
+                keep.append(g)
+            out.append(g.data_ptr())
+        return out, keep
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        keep, grads = [], []
+        for k, group in enumerate(self.param_groups):
+            if [id(p) for p in group["params"]] != [id(p) for p in self._groups[k].params]:
+                raise RuntimeError("AdamW: the parameters of a group were exchanged after the optimizer was made")
+            ptrs, more = self._gradients(k, group)
+            grads.append(ptrs)
+            keep += more
+        with ops.on_device(self._device):
+            st = ops._st()
+            nparts = ctypes.c_int32(0)
+            clip = self.max_grad_norm is not None
+            if clip:
+                numel, types, every = self._groups[0].at.numel, self._groups[0].at.types, grads[0]
+                for g, ptrs in zip(self._groups[1:], grads[1:]):
+                    numel, types, every = numel + g.at.numel, types + g.at.types, every + ptrs
+                call("m3d_grad_norm", every.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0], len(every),
+                     self._parts.data_ptr(), ctypes.addressof(nparts), st)
+            for g, group, ptrs in zip(self._groups, self.param_groups, grads):
+                self._check_group(group, self.state_bits)
+                lr = group["lr"]
+                dev_lr = isinstance(lr, Tensor)
+                params = array("Q", [p.data_ptr() for p in g.params])
+                args = _lib.M3DAdamW(
+                    params.buffer_info()[0], ptrs.buffer_info()[0], *g.at.args, self.state_bits, g.avg.data_ptr(), g.avg_sq.data_ptr(),
+                    None if g.scale is None else g.scale.data_ptr(), None if g.scale is None else g.scale_sq.data_ptr(), g.state.data_ptr(),
+                    g.missed.data_ptr(), self._parts.data_ptr() if clip else None, nparts.value, self.max_grad_norm or 0.0,
+                    self.grad_norm.data_ptr() if clip else None, lr.data_ptr() if dev_lr else None, 0.0 if dev_lr else float(lr),
+                    float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]), float(group["weight_decay"]))
+                call("m3d_adamw_step", ctypes.addressof(args), st)
+                # (the parameters changed behind torch's back: caches that go by their version counters notice)
+                torch.autograd.graph.increment_version(g.params)
+        return loss
+
+    # ------------------------------------------------------------------------------------------
+    def moments(self) -> List[Tuple[Tensor, Tensor]]:
+        """``(exp_avg, exp_avg_sq)`` of every parameter group as flat fp32 buffers: the tensors in order, each from a multiple of 256
+        elements on.  With 32 bits the optimizer's own buffers, with 8 bits the values that the codes stand for."""
+        return [g.decoded() for g in self._groups]
+
+    def state_dict(self):
+        state: Dict[int, dict] = {}
+        groups = []
+        for g, group in zip(self._groups, self.param_groups):
+            steps = (g.state[:1] - g.missed.to(torch.float32)).cpu()
+            index = list(range(len(state), len(state) + len(g.params)))
+            for i, key in enumerate(index):
+                state[key] = {"step": steps[i].clone(), "exp_avg": g.slice(g.avg, i).clone(), "exp_avg_sq": g.slice(g.avg_sq, i).clone()}
+                if g.bits == 8:
+                    state[key] |= {"exp_avg_scale": g.blocks_of(g.scale, i).clone(), "exp_avg_sq_scale": g.blocks_of(g.scale_sq, i).clone()}
+            groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": index})
+        return {"state": state, "param_groups": groups}
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        groups, state = state_dict["param_groups"], state_dict["state"]
+        if [len(g["params"]) for g in groups] != [len(g.params) for g in self._groups]:
+            raise ValueError("loaded state dict has other parameter groups")
+        todo = []
+        for g, group in zip(self._groups, groups):
+            if group.get("amsgrad", False) or group.get("maximize", False):
+                raise ValueError("AdamW implements amsgrad=False, maximize=False only")
+            entries = [state.get(key, state.get(str(key))) for key in group["params"]]
+            coded = {("exp_avg_scale" in e) for e in entries if e}
+            for p, e in zip(g.params, entries):
+                if e and tuple(e["exp_avg"].shape) != tuple(p.shape):
+                    raise ValueError(f"optimizer state has shape {tuple(e['exp_avg'].shape)}, expected {tuple(p.shape)}")
+            if len(coded) > 1 or (True in coded and g.bits != 8):
+                raise ValueError("8-bit states go into an optimizer with state_bits=8 only")
+            todo.append((g, group, entries, True in coded))
+        for (g, group, entries, coded), mine in zip(todo, self.param_groups):
+            steps = [float(e["step"]) if e else 0.0 for e in entries]
+            top = max(steps, default=0.0)
+            if coded or g.bits == 32:
+                flat = (g.avg, g.avg_sq)
+            else:
+                flat = tuple(torch.zeros(g.blocks * BLOCK, dtype=torch.float32, device=g.avg.device) for _ in range(2))
+            for f in flat + ((g.scale, g.scale_sq) if coded else ()):
+                f.zero_()
+            for i, e in enumerate(entries):
+                if not e:  # (torch has no entry for a parameter that was never stepped)
+                    continue
+                for f, key, scale in zip(flat, ("exp_avg", "exp_avg_sq"), (g.scale, g.scale_sq)):
+                    g.slice(f, i).copy_(e[key])
+                    if coded:
+                        g.blocks_of(scale, i).copy_(e[key + "_scale"])
+            if g.bits == 8 and not coded:
+                g.encode(*flat)
+            g.state.zero_()
+            g.state[0] = top
+            g.missed.copy_(torch.tensor([int(top - s) for s in steps], dtype=torch.int32))
+            for k, v in group.items():
+                if k != "params" and k in mine:
+                    mine[k] = v
