@@ -540,7 +540,7 @@ int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * `grads`, `numel`, `types` (and the arrays of M3DAdamW) are HOST arrays of `count` entries read during the call: device
  * pointer of a contiguous tensor (grads: NULL = the tensor has no gradient; aligned to its element, no more), number of
  * elements, type (M3D_TYPE_*).  Any count; the pointers travel as kernel arguments, 152 tensors a launch. */
-#define M3D_GRAD_NORM_PARTS 1024
+#define M3D_GRAD_NORM_PARTS 2048
 /* parts (device fp64 [M3D_GRAD_NORM_PARTS]) <- partial sums of g^2 over all tensors, *nparts (host) <- how many of them are
  * written: the norm is the root of their sum, which m3d_clip_grads and m3d_adamw_step take themselves.  No atomics: the
  * same gradients give the same bits. */

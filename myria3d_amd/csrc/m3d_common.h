@@ -11,6 +11,12 @@
 
 #define M3D_WAVE 64
 
+// the cache in front of the memory.  A kernel whose call touches more than this once loads and stores past it (nontemporal): the lines
+// would be gone before anyone came back for them, and their write-backs cost the kernels behind
+#ifndef M3D_CACHE_BYTES
+#define M3D_CACHE_BYTES (256ll << 20)
+#endif
+
 #define M3D_CHECK_LAUNCH()                                   \
   do {                                                       \
     if (hipGetLastError() != hipSuccess) return M3D_ERR_LAUNCH; \

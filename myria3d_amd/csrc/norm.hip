@@ -19,6 +19,7 @@
 
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short h8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef unsigned short h4u __attribute__((ext_vector_type(4), aligned(2)));
 
 struct NormArgs {
   const void *x, *dy, *w, *b;
@@ -43,28 +44,50 @@ __device__ __forceinline__ void el_store(void* base, int64_t e, float v) {
   else if constexpr (TYPE == M3D_TYPE_BF16) ((unsigned short*)base)[e] = f32_to_bf16(v);
   else ((_Float16*)base)[e] = (_Float16)v;
 }
-template <int TYPE>
-__device__ __forceinline__ void vec_load(const void* base, int64_t e, float* v) {
-  if constexpr (TYPE == M3D_TYPE_F32) {
-    const f4u t = *(const f4u*)((const float*)base + e);
+typedef uint32_t u4u __attribute__((ext_vector_type(4), aligned(2)));
+// a lane's part of a row as it lies in memory: NE vectors of 16 bytes and one element of the rest
+template <int NE> struct Raw { u4u v[NE]; float rest; };
+// (ONCE: past the caches, see M3D_CACHE_BYTES)
+template <int TYPE, int NE, bool ONCE>
+__device__ __forceinline__ Raw<NE> raw_load(const void* base, int64_t row_at, int lane, int lanes, int nv, int rest, bool has_rest) {
+  Raw<NE> r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = t[j];
-  } else {
-    const h8u t = *(const h8u*)((const unsigned short*)base + e);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const unsigned short u = t[j];
-      v[j] = TYPE == M3D_TYPE_BF16 ? bf16_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
+  for (int i = 0; i < NE; ++i) {
+    const int q = lane + i * lanes;
+    r.v[i] = u4u{0u, 0u, 0u, 0u};
+    if (q < nv) {
+      const u4u* at = (const u4u*)((const char*)base + (row_at + (int64_t)q * Vec<TYPE>::N) * (16 / Vec<TYPE>::N));
+      if constexpr (ONCE) r.v[i] = __builtin_nontemporal_load(at);
+      else r.v[i] = *at;
     }
   }
+  r.rest = has_rest ? el_load<TYPE>(base, row_at + rest) : 0.f;
+  return r;
 }
-template <int TYPE>
+template <int TYPE, int NE>
+__device__ __forceinline__ void raw_values(const Raw<NE>& r, float* x) {
+  constexpr int V = Vec<TYPE>::N;
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if constexpr (TYPE == M3D_TYPE_F32) x[i * V + j] = __uint_as_float(r.v[i][j]);
+      else {
+        const unsigned short u = (unsigned short)(r.v[i][j >> 1] >> (16 * (j & 1)));
+        x[i * V + j] = TYPE == M3D_TYPE_BF16 ? __uint_as_float(j & 1 ? r.v[i][j >> 1] & 0xffff0000u : r.v[i][j >> 1] << 16)
+                                             : (float)__builtin_bit_cast(_Float16, u);
+      }
+    }
+  x[NE * V] = r.rest;
+}
+template <int TYPE, bool ONCE>
 __device__ __forceinline__ void vec_store(void* base, int64_t e, const float* v) {
   if constexpr (TYPE == M3D_TYPE_F32) {
     f4u t;
 #pragma unroll
     for (int j = 0; j < 4; ++j) t[j] = v[j];
-    *(f4u*)((float*)base + e) = t;
+    if constexpr (ONCE) __builtin_nontemporal_store(t, (f4u*)((float*)base + e));
+    else *(f4u*)((float*)base + e) = t;
   } else {
     h8u t;
 #pragma unroll
@@ -78,12 +101,38 @@ __device__ __forceinline__ void vec_store(void* base, int64_t e, const float* v)
         t[j + 1] = __builtin_bit_cast(unsigned short, (_Float16)v[j + 1]);
       }
     }
-    *(h8u*)((unsigned short*)base + e) = t;
+    if constexpr (ONCE) __builtin_nontemporal_store(t, (h8u*)((unsigned short*)base + e));
+    else *(h8u*)((unsigned short*)base + e) = t;
   }
 }
 __device__ __forceinline__ float w_load(const void* base, int64_t e, int type, float none) {
   if (!base) return none;
   return type == M3D_TYPE_F32 ? el_load<M3D_TYPE_F32>(base, e) : type == M3D_TYPE_BF16 ? el_load<M3D_TYPE_BF16>(base, e) : el_load<M3D_TYPE_F16>(base, e);
+}
+// the weights of a lane's columns (vectors of V elements, then the one of the rest)
+template <int V, int NE>
+__device__ __forceinline__ void w_loads(const void* base, int type, float none, int lane, int lanes, int nv, int rest, bool has_rest, float* w) {
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int q = lane + i * lanes;
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      float* o = w + i * V + j;
+      o[0] = o[1] = o[2] = o[3] = q < nv ? none : 0.f;
+      if (base && q < nv) {
+        if (type == M3D_TYPE_F32) {
+          const f4u t = *(const f4u*)((const float*)base + q * V + j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = t[k];
+        } else {
+          const h4u t = *(const h4u*)((const unsigned short*)base + q * V + j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = type == M3D_TYPE_BF16 ? bf16_to_f32(t[k]) : (float)__builtin_bit_cast(_Float16, (unsigned short)t[k]);
+        }
+      }
+    }
+  }
+  w[NE * V] = has_rest ? w_load(base, rest, type, none) : 0.f;
 }
 
 template <int CTRL>
@@ -95,7 +144,7 @@ template <int TPR>
 __device__ __forceinline__ float group_sum(float v) {
   v += dpp_f<0xB1>(v);                          // quad_perm [1,0,3,2]
   v += dpp_f<0x4E>(v);                          // quad_perm [2,3,0,1]
-  v += dpp_f<0x141>(v);                         // row_half_mirror: 8 lanes
+  if constexpr (TPR >= 8) v += dpp_f<0x141>(v);   // row_half_mirror: 8 lanes
   if constexpr (TPR >= 16) v += dpp_f<0x140>(v);  // row_mirror: 16 lanes
   float a, b;
   if constexpr (TPR >= 32) { xgroup_pair16(v, a, b); v = a + b; }
@@ -109,6 +158,7 @@ __device__ __forceinline__ float across_groups(float v) {
   if constexpr (TPR <= 32) { xgroup_pair32(v, a, b); v = a + b; }
   if constexpr (TPR <= 16) { xgroup_pair16(v, a, b); v = a + b; }
   if constexpr (TPR <= 8) v += dpp_f<0x128>(v);  // row_ror:8
+  if constexpr (TPR <= 4) v += dpp_f<0x124>(v);  // row_ror:4
   return v;
 }
 // a row over a whole workgroup: wave sums through LDS; `flip` alternates the two halves of red, so that one barrier a sum is enough
@@ -133,7 +183,7 @@ __device__ __forceinline__ void wg_sums(float (&v)[S], float (*red)[16][S], int&
 
 // TPR = 0: a workgroup a row (TPR = 1 024: one of that many threads, whose lanes have half the registers)
 #define NORM_THREADS(TPR) ((TPR) == 0 ? 512 : (TPR) == 1024 ? 1024 : 256)
-template <int TYPE, int TPR, int NE>
+template <int TYPE, int TPR, int NE, bool ONCE>
 __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const NormArgs A) {
   constexpr int V = Vec<TYPE>::N;
   constexpr bool IN = TPR > 0 && TPR <= 64;  // the row sits inside a wave
@@ -143,33 +193,22 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const Nor
   const int nv = A.cols / V, rest = nv * V + lane;  // full vectors of a row; this lane's element behind them
   const bool has_rest = rest < A.cols;
   float w[NE * V + 1], b[NE * V + 1];
-#pragma unroll
-  for (int i = 0; i < NE; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (lane + i * lanes) * V + j;
-      w[i * V + j] = c < nv * V ? w_load(A.w, c, A.wtype, 1.f) : 0.f;
-      b[i * V + j] = c < nv * V ? w_load(A.b, c, A.wtype, 0.f) : 0.f;
-    }
-  w[NE * V] = has_rest ? w_load(A.w, rest, A.wtype, 1.f) : 0.f;
-  b[NE * V] = has_rest ? w_load(A.b, rest, A.wtype, 0.f) : 0.f;
   const int per = IN ? 256 / G : 1;  // rows a workgroup holds at a time
+  const int64_t step = (int64_t)gridDim.x * per;
+  int64_t row = (int64_t)blockIdx.x * per + (IN ? threadIdx.x / G : 0);
+  const int64_t turns = (A.rows - (int64_t)blockIdx.x * per + step - 1) / step;  // (the same for all lanes: they swap values)
+  Raw<NE> next = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
+  w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
+  w_loads<V, NE>(A.b, A.wtype, 0.f, lane, lanes, nv, rest, has_rest, b);
   int flip = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < A.rows; r0 += (int64_t)gridDim.x * per) {
-    const int64_t row = r0 + (IN ? threadIdx.x / G : 0);
-    const bool on = row < A.rows;  // (lanes of a row that is not there take part in the lane swaps)
-    const int64_t xo = row * A.ldx;
+  for (int64_t turn = 0; turn < turns; ++turn, row += step) {
+    const bool on = row < A.rows;
     float x[NE * V + 1];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int q = lane + i * lanes;
-      if (on && q < nv) vec_load<TYPE>(A.x, xo + q * V, &x[i * V]);
-      else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[i * V + j] = 0.f;
-      }
+    raw_values<TYPE, NE>(next, x);
+    {  // the next row is on its way while this one is summed
+      const bool more = row + step < A.rows;
+      next = raw_load<TYPE, NE, ONCE>(A.x, (row + step) * A.ldx, lane, lanes, more ? nv : 0, rest, more && has_rest);
     }
-    x[NE * V] = on && has_rest ? el_load<TYPE>(A.x, xo + rest) : 0.f;
     float s[1] = {x[NE * V]};
 #pragma unroll
     for (int e = 0; e < NE * V; ++e) s[0] += x[e];
@@ -203,7 +242,7 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const Nor
           const float z = fmaf(x[i * V + j] * rstd, w[i * V + j], b[i * V + j]);
           o[j] = z > 0.f ? z : z * A.slope;
         }
-        vec_store<TYPE>(A.y, yo + q * V, o);
+        vec_store<TYPE, ONCE>(A.y, yo + q * V, o);
       }
     }
     if (has_rest) {
@@ -213,50 +252,42 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const Nor
   }
 }
 
-template <int TYPE, int TPR, int NE, bool ACT>
+template <int TYPE, int TPR, int NE, bool ACT, bool ONCE>
 __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const NormArgs A) {
   constexpr int V = Vec<TYPE>::N, E = NE * V + 1;
   constexpr bool IN = TPR > 0 && TPR <= 64;  // the row sits inside a wave
   constexpr int G = IN ? TPR : 64;
   __shared__ float red[2][16][2];
-  extern __shared__ float sums[];  // IN: [2][cols], the workgroup's dw and db
+  extern __shared__ __attribute__((aligned(16))) float sums[];  // IN: the waves' dw and db
   const int lanes = IN ? G : blockDim.x, lane = IN ? threadIdx.x & (G - 1) : threadIdx.x;
   const int nv = A.cols / V, rest = nv * V + lane;
   const bool has_rest = rest < A.cols;
-  float w[E], b[ACT ? E : 1], dw[E], db[E];  // (b only to find the sign of z again)
-#pragma unroll
-  for (int i = 0; i < NE; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (lane + i * lanes) * V + j;
-      w[i * V + j] = c < nv * V ? w_load(A.w, c, A.wtype, 1.f) : 0.f;
-      if constexpr (ACT) b[i * V + j] = c < nv * V ? w_load(A.b, c, A.wtype, 0.f) : 0.f;
-    }
-  w[E - 1] = has_rest ? w_load(A.w, rest, A.wtype, 1.f) : 0.f;
-  if constexpr (ACT) b[E - 1] = has_rest ? w_load(A.b, rest, A.wtype, 0.f) : 0.f;
+  float w[E], b[E], dw[E], db[E];  // (b only to find the sign of z again)
+  const int per = IN ? 256 / G : 1;
+  const int64_t step = (int64_t)gridDim.x * per;
+  int64_t row = (int64_t)blockIdx.x * per + (IN ? threadIdx.x / G : 0);
+  const int64_t turns = (A.rows - (int64_t)blockIdx.x * per + step - 1) / step;
+  Raw<NE> nx = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
+  Raw<NE> ng = raw_load<TYPE, NE, ONCE>(A.dy, row * A.lddy, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
+  float nmean = row < A.rows ? A.mean[row] : 0.f, nrstd = row < A.rows ? A.rstd[row] : 0.f;
+  w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
+  if constexpr (ACT) w_loads<V, NE>(A.b, A.wtype, 0.f, lane, lanes, nv, rest, has_rest, b);
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
-  const int per = IN ? 256 / G : 1;
   int flip = 0;
-  for (int64_t r0 = (int64_t)blockIdx.x * per; r0 < A.rows; r0 += (int64_t)gridDim.x * per) {
-    const int64_t row = r0 + (IN ? threadIdx.x / G : 0);
+  for (int64_t turn = 0; turn < turns; ++turn, row += step) {
     const bool on = row < A.rows;
-    const int64_t xo = row * A.ldx, go = row * A.lddy;
     float x[E], g[E];
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int q = lane + i * lanes;
-      if (on && q < nv) {
-        vec_load<TYPE>(A.x, xo + q * V, &x[i * V]);
-        vec_load<TYPE>(A.dy, go + q * V, &g[i * V]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[i * V + j] = g[i * V + j] = 0.f;
-      }
+    raw_values<TYPE, NE>(nx, x);
+    raw_values<TYPE, NE>(ng, g);
+    const float mean = nmean, rstd = nrstd;
+    {
+      const bool more = row + step < A.rows;
+      nx = raw_load<TYPE, NE, ONCE>(A.x, (row + step) * A.ldx, lane, lanes, more ? nv : 0, rest, more && has_rest);
+      ng = raw_load<TYPE, NE, ONCE>(A.dy, (row + step) * A.lddy, lane, lanes, more ? nv : 0, rest, more && has_rest);
+      nmean = more ? A.mean[row + step] : 0.f;
+      nrstd = more ? A.rstd[row + step] : 0.f;
     }
-    x[E - 1] = on && has_rest ? el_load<TYPE>(A.x, xo + rest) : 0.f;
-    g[E - 1] = on && has_rest ? el_load<TYPE>(A.dy, go + rest) : 0.f;
-    const float mean = on ? A.mean[row] : 0.f, rstd = on ? A.rstd[row] : 0.f;
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -285,7 +316,7 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = rstd * (g[i * V + j] - m0 - x[i * V + j] * m1);
-        vec_store<TYPE>(A.dx, yo + q * V, o);
+        vec_store<TYPE, ONCE>(A.dx, yo + q * V, o);
       }
     }
     if (has_rest) el_store<TYPE>(A.dx, yo + rest, rstd * (g[E - 1] - m0 - x[E - 1] * m1));
@@ -298,21 +329,32 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
       dw[e] = across_groups<G>(dw[e]);
       db[e] = across_groups<G>(db[e]);
     }
-    const int wave = threadIdx.x >> 6;
-    for (int k = 0; k < 4; ++k) {  // one wave after the other: the same order every time
-      if (wave == k && (threadIdx.x & 63) < G) {
+    const int ld = (A.cols + 3) & ~3;  // [4 waves][dw, db][ld]: every wave its own part, added in the order of the waves
+    float* mine = sums + (threadIdx.x >> 6) * 2 * ld;
+    if ((threadIdx.x & 63) < G) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int c = e == E - 1 ? rest : (lane + (e / V) * lanes) * V + e % V;
-          if (e == E - 1 ? has_rest : c < nv * V) {
-            sums[c] = k ? sums[c] + dw[e] : dw[e];
-            sums[A.cols + c] = k ? sums[A.cols + c] + db[e] : db[e];
+      for (int i = 0; i < NE; ++i)
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const int q = lane + i * lanes, e = i * V + j;
+          if (q < nv) {
+            *(float4*)(mine + q * V + j) = make_float4(dw[e], dw[e + 1], dw[e + 2], dw[e + 3]);
+            *(float4*)(mine + ld + q * V + j) = make_float4(db[e], db[e + 1], db[e + 2], db[e + 3]);
           }
         }
+      if (has_rest) {
+        mine[rest] = dw[E - 1];
+        mine[ld + rest] = db[E - 1];
       }
-      __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * A.cols; c += 256) out[c] = sums[c];
+    __syncthreads();
+    for (int c = threadIdx.x; c < A.cols; c += 256) {
+      float w4[4], b4[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { w4[k] = sums[k * 2 * ld + c]; b4[k] = sums[(k * 2 + 1) * ld + c]; }
+      out[c] = ((w4[0] + w4[1]) + w4[2]) + w4[3];
+      out[A.cols + c] = ((b4[0] + b4[1]) + b4[2]) + b4[3];
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -417,54 +459,83 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
 }
 
 // ------------------------------------------------------------------------------------------ host
-// How a row is laid over lanes: as few lanes as hold it in 16 elements each (fewer lanes: fewer steps in the sums and fewer idle
-// ones; more elements than 16 would cost the backward pass its occupancy).  tpr = 0 with threads > 0: a workgroup a row.
+// How a row is laid over lanes (V elements a vector): as few lanes as hold it in 16 elements each — fewer lanes mean fewer steps in
+// the sums and fewer idle ones, more elements a lane would cost the backward pass its occupancy.  From a workgroup a row on, the
+// backward pass takes 8 elements a lane: twice the lanes are half the rows of partial sums, which at 8 192 columns and rows weigh
+// a tenth of the data (bf16, 8 192 x 8 192: 80 + 7 us against 94 + 7 with 16 and as many workgroups, 102 + 12 with twice as
+// many; forward 53 us with 16, 77 with 8).  Rows of up to four vectors take four lanes (2 M x 32 bf16, forward: FOUR_US).
+// tpr = 0 or 1024: a workgroup a row; ne = 0: too wide for registers.
 struct NormShape { int tpr, ne, threads; };
-static NormShape norm_shape(int32_t cols, int32_t type) {
+static NormShape norm_shape(int32_t cols, int32_t type, bool bwd) {
   const int V = type == M3D_TYPE_F32 ? 4 : 8, most = 16 / V, nv = cols / V;
-  for (int tpr = 8; tpr <= 64; tpr *= 2)
-    for (int ne = 1; ne <= most; ne *= 2)
-      if (nv <= tpr * ne) return {tpr, ne, 256};
+  if (nv <= 4 && cols % V <= 4) return {4, 1, 256};
+  for (int ne = 1; ne <= most; ne *= 2)
+    if (nv <= 8 * ne) return {8, ne, 256};
+  for (int tpr = 16; tpr <= 64; tpr *= 2)
+    if (nv <= tpr * most) return {tpr, most, 256};
+  const int wide = bwd ? most / 2 : most;
   for (int threads = 128; threads <= 1024; threads *= 2)
-    for (int ne = 1; ne <= most; ne *= 2)
-      if (nv <= threads * ne) return {0, ne, threads};
+    if (nv <= threads * wide) return {threads == 1024 ? 1024 : 0, wide, threads};
+  if (nv <= 1024 * most) return {1024, most, 1024};
   return {0, 0, 1024};
 }
-static int norm_per(const NormShape& s) { return s.tpr ? 256 / s.tpr : 1; }
-// workgroups: enough for 16 waves on each of the 256 compute units, never more than there is work
-static int64_t norm_grid(const NormShape& s, int64_t rows) {
-  const int64_t most = 256 * (s.threads >= 1024 ? 2 : 1024 / s.threads), need = m3d_cdiv(rows, norm_per(s));
-  return need < most ? need : most;
+static int norm_per(const NormShape& s) { return s.tpr && s.tpr <= 64 ? 256 / s.tpr : 1; }
+// Workgroups: at most 16 waves on each of the 256 compute units (8 in the backward pass with several rows a wave, whose registers
+// allow little more and whose ends, w, b, dw and db, cost more than they hide: 241 against 259 us at 1.6 M x 64 fp32), each with
+// the same number of turns.
+static int64_t norm_grid(const NormShape& s, int64_t rows, bool bwd) {
+  const int64_t most = 256 * (bwd && s.threads == 256 && norm_per(s) > 1 ? 2 : 1024 / s.threads), need = m3d_cdiv(rows, norm_per(s));
+  return need <= most ? need : m3d_cdiv(need, m3d_cdiv(need, most));
+}
+static bool norm_once(int64_t rows, int32_t cols, int32_t type, int matrices) {
+  return (double)rows * cols * (type == M3D_TYPE_F32 ? 4 : 2) * matrices > (double)M3D_CACHE_BYTES;
 }
 
-template <int TYPE, int TPR>
-static void launch_norm(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, size_t lds, hipStream_t st) {
-#define NORM_LAUNCH(NE)                                                                                                                       \
-  if (!bwd) hipLaunchKernelGGL((layer_norm_kernel<TYPE, TPR, NE>), dim3((unsigned)grid), dim3(s.threads), 0, st, A);                          \
-  else if (A.slope != 1.f) hipLaunchKernelGGL((layer_norm_bwd_kernel<TYPE, TPR, NE, true>), dim3((unsigned)grid), dim3(s.threads), lds, st, A); \
-  else hipLaunchKernelGGL((layer_norm_bwd_kernel<TYPE, TPR, NE, false>), dim3((unsigned)grid), dim3(s.threads), lds, st, A)
-  if (s.ne == 1) { NORM_LAUNCH(1); }
-  else if (s.ne == 2) { NORM_LAUNCH(2); }
-  else if constexpr (TYPE == M3D_TYPE_F32) { NORM_LAUNCH(4); }
-#undef NORM_LAUNCH
+template <int TYPE, int TPR, int NE, bool ONCE>
+static void launch_norm(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, hipStream_t st) {
+  const dim3 g((unsigned)grid), t(s.threads);
+  constexpr int most = 16 / Vec<TYPE>::N;
+  if (!bwd) {
+    if constexpr ((TPR > 0 && TPR <= 64) || NE == most) hipLaunchKernelGGL((layer_norm_kernel<TYPE, TPR, NE, ONCE>), g, t, 0, st, A);
+    return;
+  }
+  if constexpr (TPR != 0 || NE == most / 2) {
+    const size_t lds = TPR > 0 && TPR <= 64 && A.parts ? 4 * 2 * sizeof(float) * (size_t)((A.cols + 3) & ~3) : 0;
+    if (A.slope != 1.f) hipLaunchKernelGGL((layer_norm_bwd_kernel<TYPE, TPR, NE, true, ONCE>), g, t, lds, st, A);
+    else hipLaunchKernelGGL((layer_norm_bwd_kernel<TYPE, TPR, NE, false, ONCE>), g, t, lds, st, A);
+  }
 }
-template <int TYPE>
-static void launch_norm_type(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, hipStream_t st) {
-  const size_t lds = bwd && s.tpr && A.parts ? 2 * sizeof(float) * (size_t)A.cols : 0;
+template <int TYPE, bool ONCE>
+static void launch_norm_shape(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, hipStream_t st) {
+  constexpr int most = 16 / Vec<TYPE>::N;
   if (s.ne == 0) {
     if (bwd) hipLaunchKernelGGL(layer_norm_wide_bwd_kernel<TYPE>, dim3((unsigned)grid), dim3(1024), 0, st, A);
     else hipLaunchKernelGGL(layer_norm_wide_kernel<TYPE>, dim3((unsigned)grid), dim3(1024), 0, st, A);
     return;
   }
   switch (s.tpr) {
-    case 8: launch_norm<TYPE, 8>(A, s, grid, bwd, lds, st); break;
-    case 16: launch_norm<TYPE, 16>(A, s, grid, bwd, lds, st); break;
-    case 32: launch_norm<TYPE, 32>(A, s, grid, bwd, lds, st); break;
-    case 64: launch_norm<TYPE, 64>(A, s, grid, bwd, lds, st); break;
+    case 4: launch_norm<TYPE, 4, 1, ONCE>(A, s, grid, bwd, st); break;
+    case 8:
+      if (s.ne == 1) launch_norm<TYPE, 8, 1, ONCE>(A, s, grid, bwd, st);
+      else if (s.ne == 2) launch_norm<TYPE, 8, 2, ONCE>(A, s, grid, bwd, st);
+      else if constexpr (most == 4) launch_norm<TYPE, 8, 4, ONCE>(A, s, grid, bwd, st);
+      break;
+    case 16: launch_norm<TYPE, 16, most, ONCE>(A, s, grid, bwd, st); break;
+    case 32: launch_norm<TYPE, 32, most, ONCE>(A, s, grid, bwd, st); break;
+    case 64: launch_norm<TYPE, 64, most, ONCE>(A, s, grid, bwd, st); break;
+    case 1024:
+      if (s.ne == most) launch_norm<TYPE, 1024, most, ONCE>(A, s, grid, bwd, st);
+      else launch_norm<TYPE, 1024, most / 2, ONCE>(A, s, grid, bwd, st);
+      break;
     default:
-      if (s.threads > 512) launch_norm<TYPE, 1024>(A, s, grid, bwd, lds, st);
-      else launch_norm<TYPE, 0>(A, s, grid, bwd, lds, st);
+      if (bwd) launch_norm<TYPE, 0, most / 2, ONCE>(A, s, grid, bwd, st);
+      else launch_norm<TYPE, 0, most, ONCE>(A, s, grid, bwd, st);
   }
+}
+template <int TYPE>
+static void launch_norm_type(const NormArgs& A, const NormShape& s, int64_t grid, bool bwd, hipStream_t st) {
+  if (norm_once(A.rows, A.cols, TYPE, bwd ? 3 : 2)) launch_norm_shape<TYPE, true>(A, s, grid, bwd, st);
+  else launch_norm_shape<TYPE, false>(A, s, grid, bwd, st);
 }
 static int launch_norm_any(const NormArgs& A, const NormShape& s, int64_t grid, int32_t type, bool bwd, hipStream_t st) {
   if (type == M3D_TYPE_F32) launch_norm_type<M3D_TYPE_F32>(A, s, grid, bwd, st);
@@ -485,13 +556,13 @@ extern "C" int m3d_layer_norm_fwd(const void* x, int64_t ldx, const void* w, con
   NormArgs A{};
   A.x = x; A.w = w; A.b = b; A.y = y; A.mean = mean; A.rstd = rstd; A.rows = rows; A.ldx = ldx; A.cols = cols; A.wtype = wtype;
   A.eps = eps; A.slope = slope; A.inv = 1.f / (float)cols;
-  const NormShape s = norm_shape(cols, type);
-  return launch_norm_any(A, s, norm_grid(s, rows), type, false, (hipStream_t)stream);
+  const NormShape s = norm_shape(cols, type, false);
+  return launch_norm_any(A, s, norm_grid(s, rows, false), type, false, (hipStream_t)stream);
 }
 
 extern "C" size_t m3d_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t type) {
   if (rows <= 0 || cols < 1 || !norm_type_ok(type)) return 0;
-  return (size_t)norm_grid(norm_shape(cols, type), rows) * 2 * (size_t)cols * sizeof(float);
+  return (size_t)norm_grid(norm_shape(cols, type, true), rows, true) * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* b, const float* mean,
@@ -507,8 +578,8 @@ extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, i
   A.x = x; A.dy = dy; A.w = w; A.b = b; A.dx = dx; A.mean = (float*)mean; A.rstd = (float*)rstd; A.rows = rows; A.ldx = ldx; A.lddy = lddy;
   A.cols = cols; A.wtype = wtype; A.slope = slope; A.inv = 1.f / (float)cols;
   A.parts = (dw || db) ? (float*)ws : nullptr;
-  const NormShape s = norm_shape(cols, type);
-  const int64_t grid = norm_grid(s, rows);
+  const NormShape s = norm_shape(cols, type, true);
+  const int64_t grid = norm_grid(s, rows, true);
   if (rows > 0 && (dx || A.parts)) {
     const int rc = launch_norm_any(A, s, grid, type, true, st);
     if (rc != M3D_OK) return rc;

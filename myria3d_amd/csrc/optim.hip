@@ -21,7 +21,18 @@
 
 #define OPT_TENSORS 152   // 24 bytes each: the list stays under 4 KB of kernel arguments (HipRandLANet has 141 tensors: one launch)
 #define OPT_BLOCK 256     // elements of a block (and of one 8-bit scale)
+#ifndef OPT_PARTS
 #define OPT_PARTS M3D_GRAD_NORM_PARTS
+#endif
+#ifndef OPT_CHUNK
+#define OPT_CHUNK 32      // blocks a workgroup takes at a time where there are many: 16 or 32 KB, one run of memory
+#endif
+#ifndef OPT_PREFETCH
+#define OPT_PREFETCH (BITS == 32)
+#endif
+#ifndef OPT_GRID
+#define OPT_GRID(BITS) ((BITS) == 32 ? 1024 : 2048)
+#endif
 
 struct TensorList {
   void* p[OPT_TENSORS];
@@ -47,23 +58,6 @@ __device__ __forceinline__ float load1(const void* base, int64_t e, int type) {
 __device__ __forceinline__ void store1(void* base, int64_t e, int type, float v) {
   if (type == 0) ((float*)base)[e] = v;
   else ((unsigned short*)base)[e] = f32_to_bits(v, type);
-}
-// n (1 .. 4) elements from e on; elements beyond n come back as zeros
-__device__ __forceinline__ void load4(const void* base, int64_t e, int n, int type, float (&v)[4]) {
-  if (n >= 4) {
-    if (type == 0) {
-      const f4u t = *(const f4u*)((const float*)base + e);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = t[j];
-    } else {
-      const h4u t = *(const h4u*)((const unsigned short*)base + e);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = bits_to_f32(t[j], type);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = j < n ? load1(base, e + j, type) : 0.f;
-  }
 }
 __device__ __forceinline__ void store4(void* base, int64_t e, int n, int type, const float (&v)[4]) {
   if (n >= 4) {
@@ -139,7 +133,7 @@ __device__ __forceinline__ double range_squares(const void* base, int64_t lo, in
     }
   };
   int64_t i = threadIdx.x;
-  for (; i + 3 * 256 < n; i += 4 * 256) {
+  for (; i + (4 - 1) * 256 < n; i += 4 * 256) {
     float x[4][N];
 #pragma unroll
     for (int u = 0; u < 4; ++u) load(i + u * 256, x[u]);
@@ -156,12 +150,11 @@ __device__ __forceinline__ double range_squares(const void* base, int64_t lo, in
 
 __global__ __launch_bounds__(256) void grad_norm_kernel(const TensorList L, uint32_t chunk, double* __restrict__ parts, int add) {
   __shared__ double red[4];
-  const uint32_t end = L.blk[L.count];
+  const uint32_t first = L.blk[0], n = L.blk[L.count] - first;
   double s = 0.0;
-  uint64_t c0 = (uint64_t)L.blk[0] + (uint64_t)blockIdx.x * chunk;
-  if (c0 < end) {
-    const uint32_t c1 = c0 + chunk < end ? (uint32_t)(c0 + chunk) : end;
-    uint32_t b = (uint32_t)c0;
+  for (uint64_t c = (uint64_t)blockIdx.x * chunk; c < n; c += (uint64_t)gridDim.x * chunk) {
+    uint32_t b = first + (uint32_t)c;
+    const uint32_t c1 = first + (c + chunk < n ? (uint32_t)(c + chunk) : n);
     for (int t = tensor_of(L, b); b < c1; ++t) {
       const uint32_t stop = L.blk[t + 1] < c1 ? L.blk[t + 1] : c1;
       if (L.g[t]) {
@@ -170,8 +163,8 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const TensorList L, uint
         int64_t hi = (int64_t)(stop - L.blk[t]) * OPT_BLOCK;
         const int64_t all = tensor_numel(L, t);
         if (hi > all) hi = all;
-        const int64_t per = type == 0 ? 4 : 8, n = (hi - lo) / per, tail = lo + n * per;
-        s += type == 0 ? range_squares<0>(L.g[t], lo, n) : type == 1 ? range_squares<1>(L.g[t], lo, n) : range_squares<2>(L.g[t], lo, n);
+        const int64_t per = type == 0 ? 4 : 8, m = (hi - lo) / per, tail = lo + m * per;
+        s += type == 0 ? range_squares<0>(L.g[t], lo, m) : type == 1 ? range_squares<1>(L.g[t], lo, m) : range_squares<2>(L.g[t], lo, m);
         if (tail + (int64_t)threadIdx.x < hi) {
           const double x = (double)load1(L.g[t], tail + threadIdx.x, type);
           s = fma(x, x, s);
@@ -186,34 +179,63 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const TensorList L, uint
 
 // ---- g *= k in place (always written, as the gradients' new values).  The runs are taken in the opposite order of the norm's
 // pass: what that pass read last is still in the 256 MB cache in front of the memory.
+template <int TYPE>
+__device__ __forceinline__ void range_scale(void* base, int64_t lo, int64_t n, float k) {  // n vectors of 16 bytes from element lo on
+  constexpr int N = TYPE == 0 ? 4 : 8;
+  for (int64_t i = threadIdx.x; i < n; i += 4 * 256) {
+    f4u f[4];
+    h8u h[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * 256 < n) {
+        if constexpr (TYPE == 0) f[u] = *(const f4u*)((const float*)base + lo + (i + u * 256) * N);
+        else h[u] = *(const h8u*)((const unsigned short*)base + lo + (i + u * 256) * N);
+      }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * 256 < n) {
+        if constexpr (TYPE == 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[u][j] *= k;
+          *(f4u*)((float*)base + lo + (i + u * 256) * N) = f[u];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[u][j] = f32_to_bits(bits_to_f32(h[u][j], TYPE) * k, TYPE);
+          *(h8u*)((unsigned short*)base + lo + (i + u * 256) * N) = h[u];
+        }
+      }
+  }
+}
+
 __global__ __launch_bounds__(256) void grad_clip_kernel(const TensorList L, uint32_t chunk, const double* __restrict__ parts, int nparts,
                                                         double max_norm, float* __restrict__ norm_out) {
   __shared__ double red[4];
   const double norm = norm_of(parts, nparts, red);
   const float k = (float)clip_factor(norm, max_norm);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-  const uint32_t end = L.blk[L.count];
-  const uint64_t c0 = (uint64_t)L.blk[0] + (uint64_t)(gridDim.x - 1 - blockIdx.x) * chunk;
-  if (c0 >= end) return;
-  const uint32_t c1 = c0 + chunk < end ? (uint32_t)(c0 + chunk) : end;
-  uint32_t b = (uint32_t)c0;
-  for (int t = tensor_of(L, b); b < c1; ++t) {
-    const uint32_t stop = L.blk[t + 1] < c1 ? L.blk[t + 1] : c1;
-    if (L.g[t]) {
-      const int type = (L.info[t] >> 8) & 3;
-      int64_t hi = (int64_t)(stop - L.blk[t]) * OPT_BLOCK;
-      const int64_t all = tensor_numel(L, t);
-      if (hi > all) hi = all;
-      for (int64_t e = (int64_t)(b - L.blk[t]) * OPT_BLOCK + threadIdx.x * 4; e < hi; e += 1024) {
-        const int n = hi - e < 4 ? (int)(hi - e) : 4;
-        float v[4];
-        load4(L.g[t], e, n, type, v);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= k;
-        store4(L.g[t], e, n, type, v);
+  const uint32_t first = L.blk[0], n = L.blk[L.count] - first;
+  const int64_t chunks = ((int64_t)n + chunk - 1) / chunk;
+  for (int64_t q = chunks - 1 - blockIdx.x; q >= 0; q -= gridDim.x) {
+    const uint64_t c = (uint64_t)q * chunk;
+    uint32_t b = first + (uint32_t)c;
+    const uint32_t c1 = first + (c + chunk < n ? (uint32_t)(c + chunk) : n);
+    for (int t = tensor_of(L, b); b < c1; ++t) {
+      const uint32_t stop = L.blk[t + 1] < c1 ? L.blk[t + 1] : c1;
+      if (L.g[t]) {
+        const int type = (L.info[t] >> 8) & 3;
+        const int64_t lo = (int64_t)(b - L.blk[t]) * OPT_BLOCK;
+        int64_t hi = (int64_t)(stop - L.blk[t]) * OPT_BLOCK;
+        const int64_t all = tensor_numel(L, t);
+        if (hi > all) hi = all;
+        const int64_t per = type == 0 ? 4 : 8, m = (hi - lo) / per, tail = lo + m * per;
+        if (type == 0) range_scale<0>(L.g[t], lo, m, k);
+        else if (type == 1) range_scale<1>(L.g[t], lo, m, k);
+        else range_scale<2>(L.g[t], lo, m, k);
+        if (tail + (int64_t)threadIdx.x < hi)
+          store1(L.g[t], tail + threadIdx.x, type, load1(L.g[t], tail + threadIdx.x, type) * k);
       }
+      b = stop;
     }
-    b = stop;
   }
 }
 
@@ -246,80 +268,174 @@ __device__ __forceinline__ AdamStep adam_step_of(const AdamArgs& A, double t, do
   return s;
 }
 
-// e4m3 (OCP: 4 bits of exponent, 3 of fraction) through the conversion instructions, which round to nearest even; a value comes
-// as a double, and its conversion to 32 bits must not round to a border: the upper word's last bit takes in whether anything is
-// below it, which leaves 16 bits more than the code has.
-__device__ __forceinline__ float sticky_f32(double x) {
-  const int lo = __double2loint(x);
-  return (float)__hiloint2double(__double2hiint(x) | (lo != 0 ? 1 : 0), 0);
-}
+// ---- 8 bits.  A value comes as a double over its block's scale.  What is below the fraction's bits decides the rounding, and must
+// not be rounded itself before: the upper word's last bit takes in whether anything is below it (the words hold 17 and 16 bits more
+// than the codes do).
 #define NAN_M 0x7fu
 #define NAN_V 0xffu
-#define MIN_SCALE 1.17549435e-38f  // 2^-126
-// decoded, as held: one product in 32 bits
+__device__ __forceinline__ int sticky_word(double x) { return __double2hiint(x) | (__double2loint(x) != 0 ? 1 : 0); }
+// decoded, as held: one rounding in 32 bits (the factor 2^-8 is exact: the block's largest magnitude has code 256)
 __device__ __forceinline__ void decode_m4(uint32_t c, float s, float (&m)[4]) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-  const float k = 0.00390625f;  // 2^-8: the block's largest magnitude is code 256
+  const float k = 0.00390625f;
   m[0] = a[0] * k * s; m[1] = a[1] * k * s; m[2] = b[0] * k * s; m[3] = b[1] * k * s;
 }
 // u(c) = 2^((c >> 3) - 31) (1 + (c & 7) / 8): the code is the upper part of a float with its exponent moved
-__device__ __forceinline__ float decode_v(uint32_t c, float s) {
-  const float u = __uint_as_float((c << 20) + ((127u - 31u) << 23)) * s;
-  return c == 0u ? 0.f : c == NAN_V ? __builtin_nanf("") : u;
-}
-// what a block's largest finite magnitude is, in every lane of its wave
-__device__ __forceinline__ float wave_max_f(float v) {
-  const int i0 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false);
-  v = fmaxf(v, __int_as_float(i0));
-  const int i1 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false);
-  v = fmaxf(v, __int_as_float(i1));
-  const int i2 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false);
-  v = fmaxf(v, __int_as_float(i2));
-  const int i3 = __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false);
-  v = fmaxf(v, __int_as_float(i3));
-  return xgroup_max(v, opaque_pinf());
-}
-__device__ __forceinline__ bool finite_f(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
-
-// one wave's block of new moments -> codes and scales (every lane: four consecutive elements)
-__device__ __forceinline__ void encode_block(const double (&m)[4], const double (&v)[4], uint32_t& cm, uint32_t& cv, float& sm, float& sv) {
-  float mx = 0.f, vx = 0.f;
-  bool fm[4], fv[4];
+__device__ __forceinline__ void decode_v4(uint32_t q, float s, float (&v)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = fabsf((float)m[j]), b = (float)v[j];  // (rounding keeps the order: the largest one's rounding is the scale)
-    fm[j] = finite_f(a); fv[j] = finite_f(b);
-    mx = fmaxf(mx, fm[j] ? a : 0.f);
-    vx = fmaxf(vx, fv[j] ? b : 0.f);
+    const uint32_t c = (q >> (8 * j)) & 255u;
+    v[j] = c ? __uint_as_float((c << 20) + ((127u - 31u) << 23)) * s : 0.f;
   }
-  sm = wave_max_f(mx);
-  sv = wave_max_f(vx);
-  if (sm < MIN_SCALE) sm = 0.f;
-  if (sv < MIN_SCALE) sv = 0.f;
+  if (((~q - 0x01010101u) & q & 0x80808080u) != 0u) {  // (a byte of ones)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (((q >> (8 * j)) & 255u) == NAN_V) v[j] = __builtin_nanf("");
+  }
+}
+// the largest of a wave's values, in every lane; the bits of floats that are not negative are ordered as the floats are
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false); }
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+  v = umax(v, dpp_u<0xB1>(v));
+  v = umax(v, dpp_u<0x4E>(v));
+  v = umax(v, dpp_u<0x141>(v));
+  v = umax(v, dpp_u<0x140>(v));
+  const m3d_u2 a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = umax(a[0], a[1]);
+  const m3d_u2 b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(umax(b[0], b[1]));
+}
+
+// one wave's block of new moments (mf, vf: rounded to 32 bits) -> codes and scales; every lane: four consecutive elements
+__device__ __forceinline__ void encode_block(const double (&m)[4], const double (&v)[4], const float (&mf)[4], const float (&vf)[4],
+                                             uint32_t& cm, uint32_t& cv, float& sm, float& sv) {
+  const uint32_t inf = 0x7f800000u;
+  uint32_t mx = 0u, vx = 0u;  // (rounding keeps the order: the largest one's rounding is the scale)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    mx = umax(mx, __float_as_uint(mf[j]) & 0x7fffffffu);
+    vx = umax(vx, __float_as_uint(vf[j]) & 0x7fffffffu);
+  }
+  mx = wave_umax(mx);
+  vx = wave_umax(vx);
+  const bool odd = mx >= inf || vx >= inf;  // something is not finite: the scale is the largest of the rest
+  if (odd) {
+    asm volatile("" ::: );  // (a branch, not selects: here and below)
+    mx = vx = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = __float_as_uint(mf[j]) & 0x7fffffffu, b = __float_as_uint(vf[j]) & 0x7fffffffu;
+      mx = umax(mx, a < inf ? a : 0u);
+      vx = umax(vx, b < inf ? b : 0u);
+    }
+    mx = wave_umax(mx);
+    vx = wave_umax(vx);
+  }
+  mx = mx < 0x00800000u ? 0u : mx;  // under 2^-126
+  vx = vx < 0x00800000u ? 0u : vx;
+  sm = __uint_as_float(mx);
+  sv = __uint_as_float(vx);
+  // Quotients by the reciprocal: off by two units in the last place at most, which matters for a code only where the quotient's lower
+  // word is next to zero.  There (one value in 2^29) the division itself decides.  A scale of zero makes everything zero.
+  const double dm = (double)sm * 0.00390625, dv = (double)sv, im = mx ? 1.0 / dm : 0.0, iv = vx ? 1.0 / dv : 0.0;
+  double qm[4], qv[4];
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    qm[j] = m[j] * im;
+    qv[j] = v[j] * iv;
+    near |= (uint32_t)__double2loint(qm[j]) + 4u < 8u && m[j] != 0.0;
+    near |= (uint32_t)__double2loint(qv[j]) + 4u < 8u && v[j] != 0.0;
+  }
+  if (__ballot(near) != 0ull) {  // (a branch of the wave: the compiler would divide everywhere and select)
+    asm volatile("" ::: );
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      qm[j] = mx ? m[j] / dm : 0.0;
+      qv[j] = vx ? v[j] / dv : 0.0;
+    }
+  }
   float r[4];
   uint32_t c[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    r[j] = fm[j] && sm > 0.f ? sticky_f32(m[j] / (double)sm * 256.0) : 0.f;
-    const double q = sv > 0.f ? v[j] / (double)sv : 0.0;
-    const uint32_t u = __float_as_uint(sticky_f32(q));
-    int k = (int)((u + 0x7ffffu + ((u >> 20) & 1u)) >> 20) - ((127 - 31) << 3);  // nearest even at three bits of fraction
-    k = k < 1 ? 1 : k;                                                            // what is above zero stays above it
-    c[j] = !fv[j] ? NAN_V : q > 0.0 ? (uint32_t)k : 0u;
+    r[j] = (float)__hiloint2double(sticky_word(qm[j]), 0);  // (exact; the conversion below rounds to nearest even)
+    const uint32_t u = (uint32_t)sticky_word(qv[j]);
+    const int k = (int)((u + 0xffffu + ((u >> 17) & 1u)) >> 17) - ((1023 - 31) << 3);  // nearest even at three bits of fraction
+    c[j] = u ? (uint32_t)(k < 1 ? 1 : k) : 0u;                                         // what is above zero stays above it
   }
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], w, true);
   cm = (uint32_t)w;
+  if (odd) {
+    asm volatile("" ::: );
 #pragma unroll
-  for (int j = 0; j < 4; ++j) cm = fm[j] ? cm : (cm & ~(0xffu << (8 * j))) | (NAN_M << (8 * j));
+    for (int j = 0; j < 4; ++j) {
+      if ((__float_as_uint(mf[j]) & 0x7fffffffu) >= inf) cm = (cm & ~(0xffu << (8 * j))) | (NAN_M << (8 * j));
+      if ((__float_as_uint(vf[j]) & 0x7fffffffu) >= inf) c[j] = NAN_V;  // (the others are 248 at most)
+    }
+  }
   cv = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
 }
 
-// A workgroup's four waves take the blocks of its run in turn, a lane four consecutive elements (16-byte accesses in fp32).
-template <int BITS>
+// sqrt and quotient by the instructions (each within one unit in the last place; the update is a small part of the parameter):
+// what the compiler makes of sqrtf and / costs 25 instructions an element.  The square root's argument is kept out of the denormals.
+__device__ __forceinline__ float quick_sqrt(float v) {
+  const bool tiny = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v);
+  return tiny ? r * 0x1p-32f : r;
+}
+
+// a lane's four elements as they lie in memory
+struct Raw { uint32_t w[4]; };
+typedef uint32_t u4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u2u __attribute__((ext_vector_type(2), aligned(2)));
+template <bool ONCE>
+__device__ __forceinline__ Raw raw_load(const void* base, int64_t e, int n, int type) {
+  Raw r{};
+  if (n >= 4) {
+    if (type == 0) {
+      const u4u* at = (const u4u*)((const float*)base + e);
+      u4u t;
+      if constexpr (ONCE) t = __builtin_nontemporal_load(at);
+      else t = *at;
+      r.w[0] = t[0]; r.w[1] = t[1]; r.w[2] = t[2]; r.w[3] = t[3];
+    } else {
+      const u2u* at = (const u2u*)((const unsigned short*)base + e);
+      u2u t;
+      if constexpr (ONCE) t = __builtin_nontemporal_load(at);
+      else t = *at;
+      r.w[0] = t[0]; r.w[1] = t[1];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < n) {
+        if (type == 0) r.w[j] = ((const uint32_t*)base)[e + j];
+        else r.w[j >> 1] |= (uint32_t)((const unsigned short*)base)[e + j] << (16 * (j & 1));
+      }
+  }
+  return r;
+}
+__device__ __forceinline__ void raw_values(const Raw& r, int type, float (&v)[4]) {
+  if (type == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(r.w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = bits_to_f32((unsigned short)(r.w[j >> 1] >> (16 * (j & 1))), type);
+  }
+}
+
+// A wave takes every (number of waves)-th block, a lane four consecutive elements of it (16-byte accesses in fp32): all waves together
+// walk one window of memory.  The next block is on its way while the present one is computed.
+// ONCE: past the caches (see M3D_CACHE_BYTES), but for what is written of the parameters, which the forward pass reads next.
+template <int BITS, bool ONCE>
 __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const AdamArgs A) {
   __shared__ double red[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
   const double done = (double)__hip_atomic_load(&A.state[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   double k = 1.0;
   bool go = true;
@@ -329,55 +445,100 @@ __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const Ad
     go = norm <= 1.7e308;  // a norm that is not finite: the step is not taken (neither counted)
     if (A.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *A.norm_out = (float)norm;
   }
-  const uint32_t end = L.blk[L.count];
-  const uint64_t c0 = (uint64_t)L.blk[0] + (uint64_t)(gridDim.x - 1 - blockIdx.x) * A.chunk;  // (against the norm pass's order)
-  if (go && c0 + wave < end) {
+  const uint32_t first = L.blk[0], n = L.blk[L.count] - first, chunk = A.chunk;
+  // (chunks from the end on: against the order of the norm's pass, whose last reads are still in cache)
+  const int64_t chunks = ((int64_t)n + chunk - 1) / chunk;
+  int64_t q = chunks - 1 - blockIdx.x;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t o = wave;  // block of the chunk
+  auto there = [&]() { return q >= 0 && o < chunk && (uint64_t)q * chunk + o < n; };
+  if (go && there()) {
     const double lr = A.lr_dev ? (double)A.lr_dev[0] : A.lr;
     const float kf = (float)k, b1 = (float)A.b1, b2 = (float)A.b2, d1 = (float)A.c1, d2 = (float)A.c2;
-    const uint32_t c1 = c0 + A.chunk < end ? (uint32_t)(c0 + A.chunk) : end;
-    uint32_t b = __builtin_amdgcn_readfirstlane((uint32_t)c0 + wave);
-    if (b < c1) {
-      int t = tensor_of(L, b), at = -1;
-      AdamStep S{};
-      for (; b < c1; b += 4) {
-        while (b >= L.blk[t + 1]) ++t;
-        void* g = L.g[t];
-        if (!g) {
-          if (b == L.blk[t] && lane == 0) A.missed[L.first + t] += 1;
-          continue;
+    AdamStep S{};
+    int at = -1;
+    struct Block { int t, type, n; uint32_t b; int64_t e; bool on; } cur, nxt;
+    struct Data { Raw g, p; f32x4 m, v; uint32_t qm, qv; float sm, sv; } dc, dn;
+    auto find = [&](int t) {
+      Block r;
+      r.b = first + (uint32_t)(q * chunk + o);
+      if (t < 0 || r.b < L.blk[t] || r.b >= L.blk[t + 1]) t = tensor_of(L, r.b);
+      r.t = t;
+      r.type = (L.info[t] >> 8) & 3;
+      const int last = L.info[t] & 255;
+      r.e = (int64_t)(r.b - L.blk[t]) * OPT_BLOCK + lane * 4;
+      const int n = (r.b + 1 == L.blk[t + 1] && last ? last : OPT_BLOCK) - lane * 4;
+      r.n = n > 4 ? 4 : n;
+      r.on = L.g[t] != nullptr;
+      return r;
+    };
+    auto fetch = [&](const Block& r, Data& d) {
+      if (!r.on) return;
+      d.g = d.p = Raw{};
+      if (r.n > 0) {
+        d.g = raw_load<ONCE>(L.g[r.t], r.e, r.n, r.type);
+        d.p = raw_load<ONCE>(L.p[r.t], r.e, r.n, r.type);
+      }
+      const int64_t s = (int64_t)r.b * 64 + lane;  // the lane's four elements in the flat moments
+      if constexpr (BITS == 32) {
+        if constexpr (ONCE) {
+          d.m = __builtin_nontemporal_load(&((const f32x4*)A.m)[s]);
+          d.v = __builtin_nontemporal_load(&((const f32x4*)A.v)[s]);
+        } else {
+          d.m = ((const f32x4*)A.m)[s];
+          d.v = ((const f32x4*)A.v)[s];
         }
-        if (t != at) {
-          S = adam_step_of(A, done + 1.0 - (double)A.missed[L.first + t], lr);
-          at = t;
+      } else {
+        d.qm = ((const uint32_t*)A.m)[s];
+        d.qv = ((const uint32_t*)A.v)[s];
+        d.sm = A.ms[r.b];
+        d.sv = A.vs[r.b];
+      }
+    };
+    cur = find(-1);
+    fetch(cur, dc);
+    while (true) {
+      o += 4;
+      if (!there()) {
+        o = wave;
+        q -= gridDim.x;
+      }
+      const bool more = there();
+      if (OPT_PREFETCH && more) {
+        nxt = find(cur.t);
+        fetch(nxt, dn);
+      }
+      if (!cur.on) {
+        if (cur.b == L.blk[cur.t] && lane == 0) A.missed[L.first + cur.t] += 1;
+      } else {
+        if (cur.t != at) {
+          at = cur.t;
+          S = adam_step_of(A, done + 1.0 - (double)A.missed[L.first + at], lr);
         }
-        const int type = (L.info[t] >> 8) & 3, last = L.info[t] & 255;
-        const int64_t e = (int64_t)(b - L.blk[t]) * OPT_BLOCK + lane * 4;
-        int n = (b + 1 == L.blk[t + 1] && last ? last : OPT_BLOCK) - lane * 4;
-        n = n > 4 ? 4 : n;
-        float p[4] = {0.f, 0.f, 0.f, 0.f}, gv[4] = {0.f, 0.f, 0.f, 0.f};
-        const int64_t s = (int64_t)b * 64 + lane;  // the lane's four elements in the flat moments
-        if (n > 0) {
-          load4(g, e, n, type, gv);
-          load4(L.p[t], e, n, type, p);
-        }
-        float mf[4], vf[4];
+        const int64_t s = (int64_t)cur.b * 64 + lane;
+        float p[4], gv[4], mf[4], vf[4];
+        raw_values(dc.g, cur.type, gv);
+        raw_values(dc.p, cur.type, p);
         if constexpr (BITS == 32) {
-          const f32x4 m = ((const f32x4*)A.m)[s], v = ((const f32x4*)A.v)[s];
           f32x4 mo, vo;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float x = gv[j] * kf;
-            mf[j] = mo[j] = b1 * m[j] + d1 * x;
-            vf[j] = vo[j] = b2 * v[j] + d2 * x * x;
+            mf[j] = mo[j] = b1 * dc.m[j] + d1 * x;
+            vf[j] = vo[j] = b2 * dc.v[j] + d2 * x * x;
           }
-          ((f32x4*)A.m)[s] = mo;
-          ((f32x4*)A.v)[s] = vo;
+          if constexpr (ONCE) {
+            __builtin_nontemporal_store(mo, &((f32x4*)A.m)[s]);
+            __builtin_nontemporal_store(vo, &((f32x4*)A.v)[s]);
+          } else {
+            ((f32x4*)A.m)[s] = mo;
+            ((f32x4*)A.v)[s] = vo;
+          }
         } else {
-          const uint32_t qm = ((const uint32_t*)A.m)[s], qv = ((const uint32_t*)A.v)[s];
-          const float sm = A.ms[b], sv = A.vs[b];
-          float om[4];
+          float om[4], ov[4];
           double m[4], v[4];
-          decode_m4(qm, sm, om);
+          decode_m4(dc.qm, dc.sm, om);
+          decode_v4(dc.qv, dc.sv, ov);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             // In 64 bits, every operation rounded by itself: with decimal betas the sums (9 a + b) / 10 hit the borders of 32 bits (the
@@ -385,31 +546,38 @@ __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const Ad
 #pragma clang fp contract(off)
             const double x = (double)gv[j] * k;
             m[j] = A.b1 * (double)om[j] + A.c1 * x;
-            v[j] = A.b2 * (double)decode_v((qv >> (8 * j)) & 255u, sv) + A.c2 * (x * x);
+            v[j] = A.b2 * (double)ov[j] + A.c2 * (x * x);
             mf[j] = (float)m[j];
             vf[j] = (float)v[j];
           }
           uint32_t cm, cv;
           float nm, nv;
-          encode_block(m, v, cm, cv, nm, nv);
+          encode_block(m, v, mf, vf, cm, cv, nm, nv);
           ((uint32_t*)A.m)[s] = cm;
           ((uint32_t*)A.v)[s] = cv;
-          if (lane == 0) { A.ms[b] = nm; A.vs[b] = nv; }
+          if (lane == 0) { A.ms[cur.b] = nm; A.vs[cur.b] = nv; }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = p[j] * S.decay - S.size * mf[j] / (sqrtf(vf[j]) * S.root + A.eps);
-        if (n > 0) store4(L.p[t], e, n, type, p);
+        for (int j = 0; j < 4; ++j) p[j] = p[j] * S.decay - S.size * mf[j] * __builtin_amdgcn_rcpf(quick_sqrt(vf[j]) * S.root + A.eps);
+        if (cur.n > 0) store4(L.p[cur.t], cur.e, cur.n, cur.type, p);
       }
+      if (!more) break;
+      if (!OPT_PREFETCH) {
+        nxt = find(cur.t);
+        fetch(nxt, dn);
+      }
+      cur = nxt;
+      dc = dn;
     }
   }
   if (!A.bump) return;
   __syncthreads();  // every thread of this workgroup has used its copy of the count
   if (threadIdx.x == 0) {  // two levels of tickets: one address takes ~15 ns an arrival
     unsigned* tk = (unsigned*)&A.state[1];
-    const unsigned sub = blockIdx.x % 64, members = gridDim.x / 64 + (sub < gridDim.x % 64 ? 1u : 0u);
+    const unsigned subs = gridDim.x <= 256 ? 16 : 64, sub = blockIdx.x % subs, members = gridDim.x / subs + (sub < gridDim.x % subs ? 1u : 0u);
     if (atomicAdd(&tk[1 + sub], 1u) == members - 1) {
       tk[1 + sub] = 0u;
-      const unsigned groups = gridDim.x < 64 ? gridDim.x : 64;
+      const unsigned groups = gridDim.x < subs ? gridDim.x : subs;
       if (atomicAdd(&tk[0], 1u) == groups - 1) {
         if (go) __hip_atomic_store(&A.state[0], (float)(done + 1.0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         tk[0] = 0u;
@@ -425,10 +593,10 @@ __global__ __launch_bounds__(256) void moments_decode_kernel(const uint32_t* __r
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
     float a[4];
     decode_m4(qm[i], sm[i >> 6], a);
-    const uint32_t c = qv[i];
-    const float s = sv[i >> 6];
+    float c[4];
+    decode_v4(qv[i], sv[i >> 6], c);
     m[i] = f32x4{a[0], a[1], a[2], a[3]};
-    v[i] = f32x4{decode_v(c & 255u, s), decode_v((c >> 8) & 255u, s), decode_v((c >> 16) & 255u, s), decode_v(c >> 24, s)};
+    v[i] = f32x4{c[0], c[1], c[2], c[3]};
   }
 }
 __global__ __launch_bounds__(256) void moments_encode_kernel(const f32x4* __restrict__ m, const f32x4* __restrict__ v,
@@ -437,10 +605,11 @@ __global__ __launch_bounds__(256) void moments_encode_kernel(const f32x4* __rest
   const int lane = threadIdx.x & 63;
   for (int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); b < blocks; b += (int64_t)gridDim.x * 4) {
     const f32x4 a = m[b * 64 + lane], c = v[b * 64 + lane];
+    const float mf[4] = {a[0], a[1], a[2], a[3]}, vf[4] = {c[0], c[1], c[2], c[3]};
     const double md[4] = {a[0], a[1], a[2], a[3]}, vd[4] = {c[0], c[1], c[2], c[3]};
     uint32_t cm, cv;
     float nm, nv;
-    encode_block(md, vd, cm, cv, nm, nv);
+    encode_block(md, vd, mf, vf, cm, cv, nm, nv);
     qm[b * 64 + lane] = cm;
     qv[b * 64 + lane] = cv;
     if (lane == 0) { sm[b] = nm; sv[b] = nv; }
@@ -477,10 +646,14 @@ static int32_t fill_list(TensorList& L, void* const* params, void* const* grads,
   L.count = n;
   return i;
 }
-// blocks a workgroup takes, so that at most `most` workgroups run
-static uint32_t chunk_of(int64_t blocks, int64_t least, int64_t most) {
+// blocks a workgroup takes at a time: one where there are few (every unit then has some), up to 32, which is 16 or 32 KB
+static uint32_t chunk_of(int64_t blocks, int64_t most) {
   const int64_t c = m3d_cdiv(blocks, most);
-  return (uint32_t)(c < least ? least : c);
+  return (uint32_t)(c < 1 ? 1 : c > OPT_CHUNK ? OPT_CHUNK : c);
+}
+static int64_t grid_of(int64_t blocks, uint32_t chunk, int64_t most) {
+  const int64_t g = m3d_cdiv(blocks, chunk);
+  return g < most ? g : most;
 }
 
 extern "C" int m3d_grad_norm(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count, double* parts, int32_t* nparts,
@@ -494,7 +667,7 @@ extern "C" int m3d_grad_norm(void* const* grads, const int64_t* numel, const int
   uint32_t grid = 1;
   for (int32_t i = 0; i < count;) {
     i = fill_list(L, nullptr, grads, numel, types, i, count, 0);
-    const int64_t n = L.blk[L.count], w = m3d_cdiv(n, chunk_of(n, 1, OPT_PARTS));
+    const int64_t n = L.blk[L.count], w = grid_of(n, chunk_of(n, OPT_PARTS), OPT_PARTS);
     if (w > grid) grid = (uint32_t)w;
   }
   int32_t i = 0, add = 0;
@@ -502,8 +675,8 @@ extern "C" int m3d_grad_norm(void* const* grads, const int64_t* numel, const int
     i = count ? fill_list(L, nullptr, grads, numel, types, i, count, 0) : 0;
     if (!count) { L.count = 0; L.blk[0] = 0; L.first = 0; }
     const int64_t n = L.blk[L.count];
-    const uint32_t chunk = chunk_of(n, 1, OPT_PARTS);
-    const uint32_t gx = add ? (uint32_t)m3d_cdiv(n, chunk) : grid;
+    const uint32_t chunk = chunk_of(n, OPT_PARTS);
+    const uint32_t gx = add ? (uint32_t)grid_of(n, chunk, OPT_PARTS) : grid;
     if (gx > 0) hipLaunchKernelGGL(grad_norm_kernel, dim3(gx), dim3(256), 0, (hipStream_t)stream, L, chunk, parts, add);
     M3D_CHECK_LAUNCH();
     add = 1;
@@ -523,8 +696,8 @@ extern "C" int m3d_clip_grads(void* const* grads, const int64_t* numel, const in
     if (count) fill_list(L, nullptr, grads, numel, types, l * OPT_TENSORS, count, 0);
     else { L.count = 0; L.blk[0] = 0; L.first = 0; }
     const int64_t n = L.blk[L.count];
-    const uint32_t chunk = chunk_of(n, 1, 2048);
-    const int64_t gx = m3d_cdiv(n, chunk);
+    const uint32_t chunk = chunk_of(n, 2048);
+    const int64_t gx = grid_of(n, chunk, 2048);
     if (gx == 0 && l > 0) continue;  // (the last launch writes the norm)
     hipLaunchKernelGGL(grad_clip_kernel, dim3((unsigned)(gx > 0 ? gx : 1)), dim3(256), 0, (hipStream_t)stream, L, chunk, parts, nparts, max_norm,
                        l == 0 ? norm_out : nullptr);
@@ -553,6 +726,10 @@ extern "C" int m3d_adamw_step(const M3DAdamW* a, void* stream) {
   A.max_norm = a->max_norm; A.lr = a->lr; A.wd = a->weight_decay; A.eps = (float)a->eps;
   A.b1 = a->beta1; A.b2 = a->beta2; A.c1 = 1.0 - a->beta1; A.c2 = 1.0 - a->beta2;
   A.log_b1 = log(a->beta1); A.log_b2 = log(a->beta2);
+  double bytes = 0.0;
+  for (int32_t i = 0; i < a->count; ++i)
+    if (a->grads[i]) bytes += (double)a->numel[i] * (3 * (a->types[i] == M3D_TYPE_F32 ? 4 : 2) + (a->state_bits == 32 ? 16 : 4));
+  const bool once = bytes > (double)M3D_CACHE_BYTES;
   TensorList L;
   const int32_t lists = (int32_t)m3d_cdiv(a->count > 0 ? a->count : 1, OPT_TENSORS);
   for (int32_t l = lists - 1; l >= 0; --l) {  // (last list first: against the order of the norm's pass)
@@ -561,14 +738,21 @@ extern "C" int m3d_adamw_step(const M3DAdamW* a, void* stream) {
     if (a->count) fill_list(L, a->params, a->grads, a->numel, a->types, l * OPT_TENSORS, a->count, start);
     else { L.count = 0; L.blk[0] = 0; L.first = 0; }
     const int64_t n = (int64_t)L.blk[L.count] - L.blk[0];
-    A.chunk = chunk_of(n, 4, 2048);
     A.bump = l == 0;
     A.norm_out = l == 0 ? a->norm_out : nullptr;
-    const int64_t gx = m3d_cdiv(n, A.chunk);
+    const int64_t most = OPT_GRID(a->state_bits);
+    A.chunk = chunk_of(n, most);
+    if (A.chunk < 4) A.chunk = 4;  // (a block for every wave)
+    const int64_t gx = grid_of(n, A.chunk, most);
     if (gx == 0 && l > 0) continue;
     const dim3 grid((unsigned)(gx > 0 ? gx : 1));  // (the last launch counts the step)
-    if (a->state_bits == 32) hipLaunchKernelGGL(adamw_kernel<32>, grid, dim3(256), 0, (hipStream_t)stream, L, A);
-    else hipLaunchKernelGGL(adamw_kernel<8>, grid, dim3(256), 0, (hipStream_t)stream, L, A);
+    if (a->state_bits == 32) {
+      if (once) hipLaunchKernelGGL((adamw_kernel<32, true>), grid, dim3(256), 0, (hipStream_t)stream, L, A);
+      else hipLaunchKernelGGL((adamw_kernel<32, false>), grid, dim3(256), 0, (hipStream_t)stream, L, A);
+    } else {
+      if (once) hipLaunchKernelGGL((adamw_kernel<8, true>), grid, dim3(256), 0, (hipStream_t)stream, L, A);
+      else hipLaunchKernelGGL((adamw_kernel<8, false>), grid, dim3(256), 0, (hipStream_t)stream, L, A);
+    }
     M3D_CHECK_LAUNCH();
   }
   return M3D_OK;

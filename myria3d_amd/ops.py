@@ -1640,49 +1640,58 @@ TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # M3D_TYPE_* of
 
 def _rows_of(t: Tensor) -> Tensor:
     """``t`` as ``[rows, cols]`` with elements of a row next to each other: a view where its strides allow one."""
-    cols = t.shape[-1]
-    t = t.view(-1, cols) if t.is_contiguous() else t.reshape(-1, cols)
-    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _layer_norm_fwd(rows: Tensor, shape, w: Optional[Tensor], b: Optional[Tensor], wtype: int, eps: float, slope: float, stats: bool):
+def _layer_norm_fwd(rows: Tensor, shape, w: Optional[Tensor], b: Optional[Tensor], wtype: int, eps: float, slope: float, keep: bool):
     n, cols = rows.shape
     dev = rows.device
     y = torch.empty(shape, dtype=rows.dtype, device=dev)
-    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=dev).unbind(0) if stats else (None, None)
+    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if keep else None  # the rows' means, then 1 / deviation
+    at = stats.data_ptr() if keep else None
     with on_device(dev):
         call("m3d_layer_norm_fwd", rows.data_ptr(), rows.stride(0), _p(w), _p(b), n, cols, TYPES[rows.dtype], wtype, eps, slope,
-             y.data_ptr(), _p(mean), _p(rstd), _st())
-    return y, mean, rstd
+             y.data_ptr(), at, at and at + 4 * n, _st())
+    return y, stats
 
 
 class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, wtype, eps, slope):
         rows = _rows_of(x)
-        y, mean, rstd = _layer_norm_fwd(rows, x.shape, w, b, wtype, eps, slope, True)
-        ctx.save_for_backward(rows, w, b, mean, rstd)
+        y, stats = _layer_norm_fwd(rows, x.shape, w, b, wtype, eps, slope, True)
+        ctx.save_for_backward(rows, w, b, stats)
         ctx.args = (x.shape, wtype, slope)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        rows, w, b, mean, rstd = ctx.saved_tensors
+        # (a backward pass that is itself recorded must not pass for a constant)
+        return LayerNormFn._recorded(ctx, dy) if torch.is_grad_enabled() else LayerNormFn._gradients(ctx, dy)
+
+    @staticmethod
+    def _gradients(ctx, dy):
+        rows, w, b, stats = ctx.saved_tensors
         shape, wtype, slope = ctx.args
         n, cols = rows.shape
+        dev, xtype = rows.device, TYPES[rows.dtype]
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = _rows_of(dy)
-        dx = torch.empty(shape, dtype=rows.dtype, device=rows.device) if need_x else None
+        dx = torch.empty(shape, dtype=rows.dtype, device=dev) if need_x else None
         dw = torch.empty_like(w) if need_w else None
         db = torch.empty_like(b) if need_b else None
         ws = None
         if need_w or need_b:
-            ws = torch.empty(lib().m3d_layer_norm_bwd_workspace_bytes(n, cols, TYPES[rows.dtype]), dtype=torch.uint8, device=rows.device)
-        with on_device(rows.device):
-            call("m3d_layer_norm_bwd", dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), _p(w), _p(b), _p(mean), _p(rstd), n,
-                 cols, TYPES[rows.dtype], wtype, slope, _p(dx), _p(dw), _p(db), _p(ws), _st())
+            ws = torch.empty(lib().m3d_layer_norm_bwd_workspace_bytes(n, cols, xtype), dtype=torch.uint8, device=dev)
+        at = stats.data_ptr()
+        with on_device(dev):
+            call("m3d_layer_norm_bwd", dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), _p(w), _p(b), at, at + 4 * n, n, cols,
+                 xtype, wtype, slope, _p(dx), _p(dw), _p(db), _p(ws), _st())
         return dx, dw, db, None, None, None
+
+    _recorded = staticmethod(torch.autograd.function.once_differentiable(_gradients.__func__))
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,

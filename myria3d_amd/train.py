@@ -14,6 +14,8 @@ from __future__ import annotations
 import ctypes
 import math
 from array import array
+from itertools import repeat
+from operator import attrgetter, is_, is_not
 from typing import Dict, Iterable, List, Optional, Tuple, Union
 
 import torch
@@ -170,7 +172,7 @@ class FusedAdam(torch.optim.Optimizer):
 # many tensors at once
 # --------------------------------------------------------------------------------------------------
 BLOCK = 256  # elements of a block of the flat moments (every tensor's slice starts at a multiple of it)
-GRAD_NORM_PARTS = 1024  # M3D_GRAD_NORM_PARTS
+GRAD_NORM_PARTS = 2048  # M3D_GRAD_NORM_PARTS
 
 
 def _dense(t: Tensor) -> bool:
@@ -194,18 +196,36 @@ def _like(g: Tensor, p: Tensor) -> Tensor:
     return torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
 
 
-def _check_grad(g: Tensor) -> None:
-    if g.is_sparse or g.layout is not torch.strided:
+# (one pass over a list of tensors each, without Python code per tensor: a step over small tensors is bound by the host)
+_GRAD, _DTYPE, _LAYOUT = attrgetter("grad"), attrgetter("dtype"), attrgetter("layout")
+
+
+def _pointers(tensors: List[Tensor]) -> array:
+    return array("Q", map(Tensor.data_ptr, tensors))
+
+
+def _sizes(tensors: List[Tensor]) -> array:
+    return array("q", map(Tensor.numel, tensors))
+
+
+def _types(tensors: List[Tensor], who: str) -> array:
+    """M3D_TYPE_* of every tensor."""
+    kinds = set(map(_DTYPE, tensors))
+    for kind in kinds:
+        if kind not in ops.TYPES:
+            raise TypeError(f"{who} must be float32, bfloat16 or float16, got {kind}")
+    if len(kinds) == 1:
+        return array("i", (ops.TYPES[kinds.pop()],)) * len(tensors)
+    return array("i", map(ops.TYPES.__getitem__, map(_DTYPE, tensors)))
+
+
+def _check_strided(tensors: List[Tensor]) -> None:
+    if not set(map(_LAYOUT, tensors)) <= {torch.strided}:
         raise RuntimeError("sparse gradients are not supported")
 
 
-class _Pointers:
-    """The host arrays that the entry points read (pointers, sizes, types of a list of tensors)."""
-
-    def __init__(self, numel: Iterable[int], types: Iterable[int]):
-        self.numel, self.types = array("q", numel), array("i", types)
-        self.count = len(self.numel)
-        self.args = (self.numel.buffer_info()[0], self.types.buffer_info()[0], self.count)
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 @torch.no_grad()
@@ -219,37 +239,33 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
-    grads = [p.grad for p in params]
-    grads = [g for g in grads if g is not None]
+    grads = [g for g in map(_GRAD, params) if g is not None]
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=params[0].device if params else "cpu")
+    types = _types(grads, "clip_grad_norm_: gradients")
+    _check_strided(grads)
+    if len(set(map(Tensor.get_device, grads))) > 1:
+        raise ValueError("clip_grad_norm_: all gradients must be on one device")
+    dense = grads
+    if not all(map(Tensor.is_contiguous, grads)):
+        dense = [g if _dense(g) else g.contiguous() for g in grads]
+    ptrs, numel = _pointers(dense), _sizes(dense)
+    if len(set(ptrs)) < len(ptrs) and len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads):
+        raise ValueError("clip_grad_norm_: the same gradient twice")
     dev = grads[0].device
-    types = ops.TYPES
-    seen = set()
-    for g in grads:
-        _check_grad(g)
-        if g.device != dev:
-            raise ValueError(f"clip_grad_norm_: all gradients must be on one device, got {dev} and {g.device}")
-        if g.dtype not in types:
-            raise TypeError(f"clip_grad_norm_: gradients must be float32, bfloat16 or float16, got {g.dtype}")
-        if id(g) in seen:
-            raise ValueError("clip_grad_norm_: the same gradient twice")
-        seen.add(id(g))
     if dev.type != "cuda":
         raise RuntimeError("clip_grad_norm_ runs on an MI355X only (no CPU fallback by design)")
-    dense = [g if g.is_contiguous() or _dense(g) else g.contiguous() for g in grads]
-    at = _Pointers([g.numel() for g in dense], [types[g.dtype] for g in dense])
-    ptrs = array("Q", [g.data_ptr() for g in dense])
     parts = torch.empty(GRAD_NORM_PARTS, dtype=torch.float64, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     nparts = ctypes.c_int32(0)
     with ops.on_device(dev):
         st = ops._st()
-        call("m3d_grad_norm", ptrs.buffer_info()[0], *at.args, parts.data_ptr(), ctypes.addressof(nparts), st)
-        call("m3d_clip_grads", ptrs.buffer_info()[0], *at.args, parts.data_ptr(), nparts.value, max_norm, norm.data_ptr(), st)
-    for g, d in zip(grads, dense):
-        if d is not g:
-            g.copy_(d)
+        call("m3d_grad_norm", _at(ptrs), _at(numel), _at(types), len(ptrs), parts.data_ptr(), ctypes.addressof(nparts), st)
+        call("m3d_clip_grads", _at(ptrs), _at(numel), _at(types), len(ptrs), parts.data_ptr(), nparts.value, max_norm, norm.data_ptr(), st)
+    if dense is not grads:
+        for g, d in zip(grads, dense):
+            if d is not g:
+                g.copy_(d)
     torch.autograd.graph.increment_version(grads)
     return norm
 
@@ -259,7 +275,9 @@ class _Group:
 
     def __init__(self, params: List[Tensor], bits: int):
         self.params, self.bits = params, bits
-        self.at = _Pointers([p.numel() for p in params], [ops.TYPES[p.dtype] for p in params])
+        self.numel, self.types = _sizes(params), _types(params, "AdamW: parameters")
+        self.strides = [p.stride() for p in params]
+        self.plain = all(map(Tensor.is_contiguous, params))
         self.starts, blocks = [], 0
         for p in params:
             self.starts.append(blocks * BLOCK)
@@ -272,6 +290,11 @@ class _Group:
             self.scale, self.scale_sq = (torch.zeros(blocks, dtype=torch.float32, device=dev) for _ in range(2))
         self.state = torch.zeros(66, dtype=torch.float32, device=dev)  # (M3D_ADAM_STATE_WORDS)
         self.missed = torch.zeros(len(params), dtype=torch.int32, device=dev)
+        self.device = {params[0].get_device()}
+        self.args = _lib.M3DAdamW(numel=_at(self.numel), types=_at(self.types), count=len(params), state_bits=bits, exp_avg=self.avg.data_ptr(),
+                                  exp_avg_sq=self.avg_sq.data_ptr(), scale_avg=None if bits == 32 else self.scale.data_ptr(),
+                                  scale_avg_sq=None if bits == 32 else self.scale_sq.data_ptr(), state=self.state.data_ptr(),
+                                  missed=self.missed.data_ptr())
 
     def slice(self, flat: Tensor, i: int) -> Tensor:
         """Tensor ``i``'s part of a flat buffer, in its shape and memory order."""
@@ -372,22 +395,26 @@ class AdamW(torch.optim.Optimizer):
         self._groups.append(_Group(list(params), self.state_bits))
 
     # ------------------------------------------------------------------------------------------
-    def _gradients(self, k: int, group: dict) -> Tuple[array, List[Tensor]]:
-        """Pointers of a group's gradients (0: none) and the tensors to keep alive until they have been read."""
-        out, keep = array("Q"), []
-        for p in group["params"]:
-            g = p.grad
-            if g is None:
-                out.append(0)
-                continue
-            if g.dtype != p.dtype:
-                raise TypeError(f"AdamW: a gradient must have its parameter's type, got {g.dtype} for {p.dtype}")
-            if not (g.is_contiguous() and p.is_contiguous()):
-                _check_grad(g)
-                g = _like(g, p)
-                keep.append(g)
-            out.append(g.data_ptr())
-        return out, keep
+    def _gradients(self, g: _Group) -> Tuple[array, List[Tensor]]:
+        """Pointers of a group's gradients (0: none), and the tensors that they point to."""
+        params = g.params
+        moved = _sizes(params) != g.numel or _types(params, "AdamW: parameters") != g.types or set(map(Tensor.get_device, params)) != g.device
+        if moved or not (all(map(Tensor.is_contiguous, params)) if g.plain else [p.stride() for p in params] == g.strides):
+            raise RuntimeError("AdamW: a parameter changed its size, type, order or device after the optimizer was made")
+        grads = list(map(_GRAD, params))
+        there, numel, types = grads, g.numel, g.types
+        if not all(map(is_not, grads, repeat(None))):
+            there = [x for x in grads if x is not None]
+            numel, types = (array(a.typecode, (n for n, x in zip(a, grads) if x is not None)) for a in (numel, types))
+        _check_strided(there)
+        if _sizes(there) != numel or _types(there, "AdamW: gradients") != types:
+            raise RuntimeError("AdamW: a gradient must have its parameter's size and type")
+        if not (g.plain and all(map(Tensor.is_contiguous, there))):
+            grads = [None if x is None else _like(x, p) for x, p in zip(grads, params)]
+            there = [x for x in grads if x is not None]
+        if len(there) == len(grads):
+            return _pointers(grads), there
+        return array("Q", (0 if x is None else x.data_ptr() for x in grads)), there
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -395,35 +422,35 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        keep, grads = [], []
-        for k, group in enumerate(self.param_groups):
-            if [id(p) for p in group["params"]] != [id(p) for p in self._groups[k].params]:
+        pointers, keep = [], []
+        for g, group in zip(self._groups, self.param_groups):
+            self._check_group(group, self.state_bits)
+            if len(group["params"]) != len(g.params) or not all(map(is_, group["params"], g.params)):
                 raise RuntimeError("AdamW: the parameters of a group were exchanged after the optimizer was made")
-            ptrs, more = self._gradients(k, group)
-            grads.append(ptrs)
-            keep += more
+            ptrs, there = self._gradients(g)
+            pointers.append(ptrs)
+            keep.append(there)
+        clip = self.max_grad_norm is not None
         with ops.on_device(self._device):
             st = ops._st()
             nparts = ctypes.c_int32(0)
-            clip = self.max_grad_norm is not None
             if clip:
-                numel, types, every = self._groups[0].at.numel, self._groups[0].at.types, grads[0]
-                for g, ptrs in zip(self._groups[1:], grads[1:]):
-                    numel, types, every = numel + g.at.numel, types + g.at.types, every + ptrs
-                call("m3d_grad_norm", every.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0], len(every),
-                     self._parts.data_ptr(), ctypes.addressof(nparts), st)
-            for g, group, ptrs in zip(self._groups, self.param_groups, grads):
-                self._check_group(group, self.state_bits)
-                lr = group["lr"]
-                dev_lr = isinstance(lr, Tensor)
-                params = array("Q", [p.data_ptr() for p in g.params])
-                args = _lib.M3DAdamW(
-                    params.buffer_info()[0], ptrs.buffer_info()[0], *g.at.args, self.state_bits, g.avg.data_ptr(), g.avg_sq.data_ptr(),
-                    None if g.scale is None else g.scale.data_ptr(), None if g.scale is None else g.scale_sq.data_ptr(), g.state.data_ptr(),
-                    g.missed.data_ptr(), self._parts.data_ptr() if clip else None, nparts.value, self.max_grad_norm or 0.0,
-                    self.grad_norm.data_ptr() if clip else None, lr.data_ptr() if dev_lr else None, 0.0 if dev_lr else float(lr),
-                    float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]), float(group["weight_decay"]))
-                call("m3d_adamw_step", ctypes.addressof(args), st)
+                numel, types, grads = self._groups[0].numel, self._groups[0].types, pointers[0]
+                for g, ptrs in zip(self._groups[1:], pointers[1:]):
+                    numel, types, grads = numel + g.numel, types + g.types, grads + ptrs
+                call("m3d_grad_norm", _at(grads), _at(numel), _at(types), len(grads), self._parts.data_ptr(), ctypes.addressof(nparts), st)
+            for g, group, ptrs in zip(self._groups, self.param_groups, pointers):
+                lr, (b1, b2) = group["lr"], group["betas"]
+                a, params = g.args, _pointers(g.params)
+                a.params, a.grads = _at(params), _at(ptrs)
+                if clip:
+                    a.parts, a.nparts, a.max_norm, a.norm_out = self._parts.data_ptr(), nparts.value, self.max_grad_norm, self.grad_norm.data_ptr()
+                if isinstance(lr, Tensor):
+                    a.lr_dev, a.lr = lr.data_ptr(), 0.0
+                else:
+                    a.lr_dev, a.lr = None, lr
+                a.beta1, a.beta2, a.eps, a.weight_decay = b1, b2, group["eps"], group["weight_decay"]
+                call("m3d_adamw_step", ctypes.addressof(a), st)
                 # (the parameters changed behind torch's back: caches that go by their version counters notice)
                 torch.autograd.graph.increment_version(g.params)
         return loss

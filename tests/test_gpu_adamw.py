@@ -163,7 +163,11 @@ def held(x, table):
     s = blocks.abs().amax(1, keepdim=True).float()
     s[s < 2.0 ** -126] = 0
     r = torch.where(s > 0, blocks / s.double(), 0.0)
-    near = table[torch.bucketize(r, (table[1:] + table[:-1]) / 2)]
+    mids = (table[1:] + table[:-1]) / 2
+    at = torch.bucketize(r, mids)  # (a value between two: the lower one)
+    zero = int((table == 0).nonzero())
+    tie = (r == mids[at.clamp(max=mids.numel() - 1)]) & ((at - zero) % 2 != 0)  # half way (gradients of few bits get there): the even code
+    near = table[at + tie]
     if table[0] == 0:  # second moments: what is above zero stays above it
         near = torch.where((r > 0) & (near == 0), table[1], near)
     return (near.float() * s).view(-1)[:n].view(x.shape)
@@ -350,6 +354,18 @@ def test_small_values_zeros_and_values_that_are_not_finite(bits):
         g = torch.where(good, p.grad, 0).double()
         assert torch.equal(m[good], held((1 - 0.9) * g, table_m())[good])
         assert torch.equal(v[good], held((1 - 0.999) * (g * g), table_v())[good])
+    if bits == 8:  # (whatever stands beside them, in all places of a word)
+        q = torch.ones(300 * BLOCK, device="cuda", requires_grad=True)
+        q.grad = torch.randn(300 * BLOCK, device="cuda")
+        for k in range(4):
+            q.grad[k * BLOCK + k::4 * BLOCK] = (float("inf"), float("nan"), float("-inf"), float("nan"))[k]
+        other = myria3d_amd.AdamW([q], state_bits=8)
+        other.step()
+        (m, v), = other.moments()
+        fine = torch.isfinite(q.grad)
+        g = torch.where(fine, q.grad, 0).double()
+        assert torch.equal(m[fine], held((1 - 0.9) * g, table_m())[fine]) and torch.equal(v[fine], held((1 - 0.999) * (g * g), table_v())[fine])
+        assert bool(torch.isnan(m[~fine]).all()) and bool(torch.isnan(v[~fine]).all())
     p.grad.zero_()
     opt.step()  # the others go on
     assert bool(torch.isfinite(p[good]).all()) and bool(torch.isnan(p[~good]).all())
