@@ -462,8 +462,8 @@ __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __r
 // How a row is laid over lanes (V elements a vector): as few lanes as hold it in 16 elements each — fewer lanes mean fewer steps in
 // the sums and fewer idle ones, more elements a lane would cost the backward pass its occupancy.  From a workgroup a row on, the
 // backward pass takes 8 elements a lane: twice the lanes are half the rows of partial sums, which at 8 192 columns and rows weigh
-// a tenth of the data (bf16, 8 192 x 8 192: 80 + 7 us against 94 + 7 with 16 and as many workgroups, 102 + 12 with twice as
-// many; forward 53 us with 16, 77 with 8).  Rows of up to four vectors take four lanes (2 M x 32 bf16, forward: FOUR_US).
+// a tenth of the data (bf16, 8 192 x 8 192: 90 + 7 us against 94 + 7 with 16 and half the workgroups, 102 + 12 with as
+// many; forward 53 us with 16, 77 with 8).  Rows of up to four vectors take four lanes (2 M x 32 bf16: forward 50 us with four, 86 with eight).
 // tpr = 0 or 1024: a workgroup a row; ne = 0: too wide for registers.
 struct NormShape { int tpr, ne, threads; };
 static NormShape norm_shape(int32_t cols, int32_t type, bool bwd) {
@@ -550,6 +550,7 @@ static bool element_aligned(const void* p, int32_t type) { return (((uintptr_t)p
 extern "C" int m3d_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int64_t rows, int32_t cols, int32_t type,
                                   int32_t wtype, float eps, float slope, void* y, float* mean, float* rstd, void* stream) {
   if (rows < 0 || cols < 1 || ldx < 0 || !norm_type_ok(type) || !norm_type_ok(wtype) || !(eps >= 0.f)) return M3D_ERR_INVALID;
+  if (cols > 1 << 30) return M3D_ERR_UNSUPPORTED;  // (columns are counted in 32 bits)
   if (rows == 0) return M3D_OK;
   if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return M3D_ERR_INVALID;
   if (!element_aligned(x, type) || !element_aligned(y, type) || !element_aligned(w, wtype) || !element_aligned(b, wtype)) return M3D_ERR_INVALID;
@@ -569,6 +570,7 @@ extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, i
                                   const float* rstd, int64_t rows, int32_t cols, int32_t type, int32_t wtype, float slope, void* dx,
                                   void* dw, void* db, void* ws, void* stream) {
   if (rows < 0 || cols < 1 || ldx < 0 || lddy < 0 || !norm_type_ok(type) || !norm_type_ok(wtype)) return M3D_ERR_INVALID;
+  if (cols > 1 << 30) return M3D_ERR_UNSUPPORTED;
   if (rows > 0 && (!dy || !x || !mean || !rstd || ((dw || db) && !ws))) return M3D_ERR_INVALID;
   if (!element_aligned(x, type) || !element_aligned(dy, type) || !element_aligned(dx, type) || !element_aligned(w, wtype) ||
       !element_aligned(b, wtype) || !element_aligned(dw, wtype) || !element_aligned(db, wtype) || (((uintptr_t)ws) & 3))

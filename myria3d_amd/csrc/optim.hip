@@ -21,18 +21,9 @@
 
 #define OPT_TENSORS 152   // 24 bytes each: the list stays under 4 KB of kernel arguments (HipRandLANet has 141 tensors: one launch)
 #define OPT_BLOCK 256     // elements of a block (and of one 8-bit scale)
-#ifndef OPT_PARTS
 #define OPT_PARTS M3D_GRAD_NORM_PARTS
-#endif
-#ifndef OPT_CHUNK
 #define OPT_CHUNK 32      // blocks a workgroup takes at a time where there are many: 16 or 32 KB, one run of memory
-#endif
-#ifndef OPT_PREFETCH
-#define OPT_PREFETCH (BITS == 32)
-#endif
-#ifndef OPT_GRID
-#define OPT_GRID(BITS) ((BITS) == 32 ? 1024 : 2048)
-#endif
+#define OPT_DECODE 4      // blocks a wave decodes side by side
 
 struct TensorList {
   void* p[OPT_TENSORS];
@@ -111,8 +102,8 @@ __device__ __forceinline__ double clip_factor(double norm, double max_norm) {
   return k > 1.0 ? 1.0 : k;  // (a NaN norm stays a NaN)
 }
 
-// ---- s: fp64 partial sums of g^2 (the products and sums are exact to 2^-53: the factor that follows, and every 8-bit code
-// behind it, does not depend on how the work was cut).  One workgroup per run of blocks, four 16-byte loads in flight.
+// ---- s: fp64 partial sums of g^2 (to 2^-53: the factor that follows, and every 8-bit code behind it, does not depend on how
+// the work was cut).  Bound by memory: 400 MB fp32 in 80 us, 250 MB bf16 in 55 us where the caches held nothing to write back before.
 template <int TYPE>
 __device__ __forceinline__ double range_squares(const void* base, int64_t lo, int64_t n) {  // n vectors of 16 bytes from element lo on
   constexpr int N = TYPE == 0 ? 4 : 8;
@@ -148,7 +139,7 @@ __device__ __forceinline__ double range_squares(const void* base, int64_t lo, in
   return s[0] + s[1];
 }
 
-__global__ __launch_bounds__(256) void grad_norm_kernel(const TensorList L, uint32_t chunk, double* __restrict__ parts, int add) {
+__global__ __launch_bounds__(256, 8) void grad_norm_kernel(const TensorList L, uint32_t chunk, double* __restrict__ parts, int add) {
   __shared__ double red[4];
   const uint32_t first = L.blk[0], n = L.blk[L.count] - first;
   double s = 0.0;
@@ -177,8 +168,8 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const TensorList L, uint
   if (threadIdx.x == 0) parts[blockIdx.x] = add ? parts[blockIdx.x] + s : s;
 }
 
-// ---- g *= k in place (always written, as the gradients' new values).  The runs are taken in the opposite order of the norm's
-// pass: what that pass read last is still in the 256 MB cache in front of the memory.
+// ---- g *= k in place (written also where k = 1).  The runs are taken in the opposite order of the norm's pass: what that pass
+// read last is still in the 256 MB cache in front of the memory.  250 MB bf16: 82 us, 6.1 TB/s of reading and writing.
 template <int TYPE>
 __device__ __forceinline__ void range_scale(void* base, int64_t lo, int64_t n, float k) {  // n vectors of 16 bytes from element lo on
   constexpr int N = TYPE == 0 ? 4 : 8;
@@ -429,11 +420,18 @@ __device__ __forceinline__ void raw_values(const Raw& r, int type, float (&v)[4]
   }
 }
 
-// A wave takes every (number of waves)-th block, a lane four consecutive elements of it (16-byte accesses in fp32): all waves together
-// walk one window of memory.  The next block is on its way while the present one is computed.
+// A workgroup walks chunks of up to 32 blocks, its four waves take a chunk's blocks in turn, a lane four consecutive elements (16-byte
+// accesses in fp32); all workgroups together walk one window of memory, and a chunk's 8-bit scales, one line of cache, have one writer
+// (with single blocks dealt out to the waves of all workgroups: 590 against 440 us for 100 M parameters with 8-bit moments).
+//   32 bits: bound by memory.  The next block is on its way while the present one is computed.  75 M bf16 parameters (22 bytes each):
+//     270 us, 6.1 TB/s, what a large scaling reaches here; 3 M fp32 (28 bytes): 19.5 us.
+//   8 bits: 85 vector instructions an element, a third of them in 64 bits (whose rate is that of 32), beside 16 bytes: 100 M fp32
+//     parameters take 350 us, 4.6 TB/s, of which the instructions alone are about 220.  Fetching ahead costs more in registers than it
+//     hides (385 us).
 // ONCE: past the caches (see M3D_CACHE_BYTES), but for what is written of the parameters, which the forward pass reads next.
 template <int BITS, bool ONCE>
-__global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const AdamArgs A) {
+__global__ __launch_bounds__(256, 5) void adamw_kernel(const TensorList L, const AdamArgs A) {
+  constexpr bool AHEAD = BITS == 32;
   __shared__ double red[4];
   const int lane = threadIdx.x & 63;
   const double done = (double)__hip_atomic_load(&A.state[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -452,6 +450,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const Ad
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t o = wave;  // block of the chunk
   auto there = [&]() { return q >= 0 && o < chunk && (uint64_t)q * chunk + o < n; };
+  if (!there()) q -= gridDim.x;  // (the last chunk may hold less than a block for every wave; all others hold one)
   if (go && there()) {
     const double lr = A.lr_dev ? (double)A.lr_dev[0] : A.lr;
     const float kf = (float)k, b1 = (float)A.b1, b2 = (float)A.b2, d1 = (float)A.c1, d2 = (float)A.c2;
@@ -504,7 +503,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const Ad
         q -= gridDim.x;
       }
       const bool more = there();
-      if (OPT_PREFETCH && more) {
+      if (AHEAD && more) {
         nxt = find(cur.t);
         fetch(nxt, dn);
       }
@@ -562,7 +561,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const Ad
         if (cur.n > 0) store4(L.p[cur.t], cur.e, cur.n, cur.type, p);
       }
       if (!more) break;
-      if (!OPT_PREFETCH) {
+      if (!AHEAD) {
         nxt = find(cur.t);
         fetch(nxt, dn);
       }
@@ -589,14 +588,26 @@ __global__ __launch_bounds__(256) void adamw_kernel(const TensorList L, const Ad
 // ---- 8-bit moments <-> 32 bits (checkpoints, inspection)
 __global__ __launch_bounds__(256) void moments_decode_kernel(const uint32_t* __restrict__ qm, const uint32_t* __restrict__ qv,
                                                              const float* __restrict__ sm, const float* __restrict__ sv,
-                                                             f32x4* __restrict__ m, f32x4* __restrict__ v, int64_t n4) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
-    float a[4];
-    decode_m4(qm[i], sm[i >> 6], a);
-    float c[4];
-    decode_v4(qv[i], sv[i >> 6], c);
-    m[i] = f32x4{a[0], a[1], a[2], a[3]};
-    v[i] = f32x4{c[0], c[1], c[2], c[3]};
+                                                             f32x4* __restrict__ m, f32x4* __restrict__ v, int64_t blocks) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t b = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * OPT_DECODE; b < blocks; b += (int64_t)gridDim.x * 4 * OPT_DECODE) {
+    uint32_t cm[OPT_DECODE], cv[OPT_DECODE];
+    float fm[OPT_DECODE], fv[OPT_DECODE];
+#pragma unroll
+    for (int u = 0; u < OPT_DECODE; ++u) {  // (a wave: four blocks side by side, all on their way before the first is stored)
+      const int64_t k = b + u < blocks ? b + u : blocks - 1;
+      cm[u] = qm[k * 64 + lane]; cv[u] = qv[k * 64 + lane];
+      fm[u] = sm[k]; fv[u] = sv[k];
+    }
+#pragma unroll
+    for (int u = 0; u < OPT_DECODE; ++u) {
+      if (b + u >= blocks) break;
+      float a[4], c[4];
+      decode_m4(cm[u], fm[u], a);
+      decode_v4(cv[u], fv[u], c);
+      m[(b + u) * 64 + lane] = f32x4{a[0], a[1], a[2], a[3]};
+      v[(b + u) * 64 + lane] = f32x4{c[0], c[1], c[2], c[3]};
+    }
   }
 }
 __global__ __launch_bounds__(256) void moments_encode_kernel(const f32x4* __restrict__ m, const f32x4* __restrict__ v,
@@ -655,6 +666,11 @@ static int64_t grid_of(int64_t blocks, uint32_t chunk, int64_t most) {
   const int64_t g = m3d_cdiv(blocks, chunk);
   return g < most ? g : most;
 }
+
+// Workgroups of the update: what the registers let run at once (five waves on a SIMD; more would run behind the first ones, alone:
+// 100 M parameters with 8-bit moments take 350 us with 1 280 and 410 with 1 792).  With 32-bit moments four are enough to keep the memory
+// busy (75 M bf16 parameters: 270 us with 1 024, 276 with 1 280, 330 with 1 536).
+static int64_t adamw_grid(int32_t bits) { return bits == 32 ? 1024 : 1280; }
 
 extern "C" int m3d_grad_norm(void* const* grads, const int64_t* numel, const int32_t* types, int32_t count, double* parts, int32_t* nparts,
                              void* stream) {
@@ -740,7 +756,7 @@ extern "C" int m3d_adamw_step(const M3DAdamW* a, void* stream) {
     const int64_t n = (int64_t)L.blk[L.count] - L.blk[0];
     A.bump = l == 0;
     A.norm_out = l == 0 ? a->norm_out : nullptr;
-    const int64_t most = OPT_GRID(a->state_bits);
+    const int64_t most = adamw_grid(a->state_bits);
     A.chunk = chunk_of(n, most);
     if (A.chunk < 4) A.chunk = 4;  // (a block for every wave)
     const int64_t gx = grid_of(n, A.chunk, most);
@@ -764,10 +780,10 @@ extern "C" int m3d_moments_decode(const void* exp_avg, const void* exp_avg_sq, c
   if (blocks == 0) return M3D_OK;
   if (!exp_avg || !exp_avg_sq || !scale_avg || !scale_avg_sq || !avg_out || !avg_sq_out) return M3D_ERR_INVALID;
   if ((((uintptr_t)exp_avg) | ((uintptr_t)exp_avg_sq)) & 3 || (((uintptr_t)avg_out) | ((uintptr_t)avg_sq_out)) & 15) return M3D_ERR_INVALID;
-  int64_t gx = m3d_cdiv(blocks * 64, 256);
-  if (gx > 8192) gx = 8192;
+  int64_t gx = m3d_cdiv(blocks, 4 * OPT_DECODE);
+  if (gx > 1 << 20) gx = 1 << 20;
   hipLaunchKernelGGL(moments_decode_kernel, dim3((unsigned)gx), dim3(256), 0, (hipStream_t)stream, (const uint32_t*)exp_avg,
-                     (const uint32_t*)exp_avg_sq, scale_avg, scale_avg_sq, (f32x4*)avg_out, (f32x4*)avg_sq_out, blocks * 64);
+                     (const uint32_t*)exp_avg_sq, scale_avg, scale_avg_sq, (f32x4*)avg_out, (f32x4*)avg_sq_out, blocks);
   M3D_CHECK_LAUNCH();
   return M3D_OK;
 }

@@ -1705,8 +1705,8 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     are held in 32 bits or more; the result has ``x``'s type, the gradients their tensor's.  Same inputs, same bits."""
     if x.dtype not in TYPES:
         raise TypeError(f"layer_norm: x must be float32, bfloat16 or float16, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"layer_norm: x needs a last dimension of one element at least, got shape {tuple(x.shape)}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 30:
+        raise ValueError(f"layer_norm: x needs a last dimension of 1 to 2^30 elements, got shape {tuple(x.shape)}")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue

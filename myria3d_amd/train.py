@@ -197,7 +197,7 @@ def _like(g: Tensor, p: Tensor) -> Tensor:
 
 
 # (one pass over a list of tensors each, without Python code per tensor: a step over small tensors is bound by the host)
-_GRAD, _DTYPE, _LAYOUT = attrgetter("grad"), attrgetter("dtype"), attrgetter("layout")
+_GRAD, _DTYPE, _SPARSE = attrgetter("grad"), attrgetter("dtype"), attrgetter("is_sparse")
 
 
 def _pointers(tensors: List[Tensor]) -> array:
@@ -220,7 +220,7 @@ def _types(tensors: List[Tensor], who: str) -> array:
 
 
 def _check_strided(tensors: List[Tensor]) -> None:
-    if not set(map(_LAYOUT, tensors)) <= {torch.strided}:
+    if any(map(_SPARSE, tensors)):
         raise RuntimeError("sparse gradients are not supported")
 
 
@@ -290,7 +290,7 @@ class _Group:
             self.scale, self.scale_sq = (torch.zeros(blocks, dtype=torch.float32, device=dev) for _ in range(2))
         self.state = torch.zeros(66, dtype=torch.float32, device=dev)  # (M3D_ADAM_STATE_WORDS)
         self.missed = torch.zeros(len(params), dtype=torch.int32, device=dev)
-        self.device = {params[0].get_device()}
+        self.pointers, self.aliases = _pointers(params), [p.detach() for p in params]
         self.args = _lib.M3DAdamW(numel=_at(self.numel), types=_at(self.types), count=len(params), state_bits=bits, exp_avg=self.avg.data_ptr(),
                                   exp_avg_sq=self.avg_sq.data_ptr(), scale_avg=None if bits == 32 else self.scale.data_ptr(),
                                   scale_avg_sq=None if bits == 32 else self.scale_sq.data_ptr(), state=self.state.data_ptr(),
@@ -395,22 +395,30 @@ class AdamW(torch.optim.Optimizer):
         self._groups.append(_Group(list(params), self.state_bits))
 
     # ------------------------------------------------------------------------------------------
+    def _parameters(self, g: _Group) -> array:
+        """Pointers of a group's parameters.  The aliases made with the group keep the memory that they were found in alive: where the
+        pointers are the same, the parameters are where they were; elsewhere everything about them is looked at again."""
+        ptrs = _pointers(g.params)
+        if ptrs != g.pointers:
+            params = g.params
+            if (_sizes(params) != g.numel or _types(params, "AdamW: parameters") != g.types or [p.stride() for p in params] != g.strides
+                    or {p.get_device() for p in params} != {self._device.index}):
+                raise RuntimeError("AdamW: a parameter changed its size, type, order or device after the optimizer was made")
+            g.pointers, g.aliases = ptrs, [p.detach() for p in params]
+        return ptrs
+
     def _gradients(self, g: _Group) -> Tuple[array, List[Tensor]]:
         """Pointers of a group's gradients (0: none), and the tensors that they point to."""
-        params = g.params
-        moved = _sizes(params) != g.numel or _types(params, "AdamW: parameters") != g.types or set(map(Tensor.get_device, params)) != g.device
-        if moved or not (all(map(Tensor.is_contiguous, params)) if g.plain else [p.stride() for p in params] == g.strides):
-            raise RuntimeError("AdamW: a parameter changed its size, type, order or device after the optimizer was made")
-        grads = list(map(_GRAD, params))
+        grads = list(map(_GRAD, g.params))
         there, numel, types = grads, g.numel, g.types
         if not all(map(is_not, grads, repeat(None))):
             there = [x for x in grads if x is not None]
             numel, types = (array(a.typecode, (n for n, x in zip(a, grads) if x is not None)) for a in (numel, types))
         _check_strided(there)
-        if _sizes(there) != numel or _types(there, "AdamW: gradients") != types:
-            raise RuntimeError("AdamW: a gradient must have its parameter's size and type")
+        if _sizes(there) != numel or _types(there, "AdamW: gradients") != types or not set(map(Tensor.get_device, there)) <= {self._device.index}:
+            raise RuntimeError("AdamW: a gradient must have its parameter's size, type and device")
         if not (g.plain and all(map(Tensor.is_contiguous, there))):
-            grads = [None if x is None else _like(x, p) for x, p in zip(grads, params)]
+            grads = [None if x is None else _like(x, p) for x, p in zip(grads, g.params)]
             there = [x for x in grads if x is not None]
         if len(there) == len(grads):
             return _pointers(grads), there
@@ -427,21 +435,22 @@ class AdamW(torch.optim.Optimizer):
             self._check_group(group, self.state_bits)
             if len(group["params"]) != len(g.params) or not all(map(is_, group["params"], g.params)):
                 raise RuntimeError("AdamW: the parameters of a group were exchanged after the optimizer was made")
+            params = self._parameters(g)
             ptrs, there = self._gradients(g)
-            pointers.append(ptrs)
+            pointers.append((params, ptrs))
             keep.append(there)
         clip = self.max_grad_norm is not None
         with ops.on_device(self._device):
             st = ops._st()
             nparts = ctypes.c_int32(0)
             if clip:
-                numel, types, grads = self._groups[0].numel, self._groups[0].types, pointers[0]
-                for g, ptrs in zip(self._groups[1:], pointers[1:]):
+                numel, types, grads = self._groups[0].numel, self._groups[0].types, pointers[0][1]
+                for g, (_, ptrs) in zip(self._groups[1:], pointers[1:]):
                     numel, types, grads = numel + g.numel, types + g.types, grads + ptrs
                 call("m3d_grad_norm", _at(grads), _at(numel), _at(types), len(grads), self._parts.data_ptr(), ctypes.addressof(nparts), st)
-            for g, group, ptrs in zip(self._groups, self.param_groups, pointers):
+            for g, group, (params, ptrs) in zip(self._groups, self.param_groups, pointers):
                 lr, (b1, b2) = group["lr"], group["betas"]
-                a, params = g.args, _pointers(g.params)
+                a = g.args
                 a.params, a.grads = _at(params), _at(ptrs)
                 if clip:
                     a.parts, a.nparts, a.max_norm, a.norm_out = self._parts.data_ptr(), nparts.value, self.max_grad_norm, self.grad_norm.data_ptr()

@@ -259,6 +259,19 @@ def test_adamw_over_many_tensors_with_clipping(bits):
     assert (norm < 1.0) or scale == 1.0
 
 
+@pytest.mark.parametrize("blocks", [32 * 1290 + 1, 32 * 2100 + 3])  # several chunks of 32 blocks a workgroup; the second: past the caches
+@pytest.mark.parametrize("bits, dtype", [(32, torch.float32), (32, torch.bfloat16), (8, torch.float32), (8, torch.float16)])
+def test_adamw_over_large_tensors_whose_last_chunk_is_short(bits, dtype, blocks):
+    import myria3d_amd
+
+    params = tensors([(BLOCK * 7 - 3,), (BLOCK * (blocks - 9) - 5,), (2 * BLOCK,)], dtype, 14)
+    opt = myria3d_amd.AdamW(params, state_bits=bits, max_grad_norm=10.0)
+    counts = [0] * 3
+    for _ in range(2):
+        k = min(1.0, 10.0 / (float(grads_of(params).square().sum().sqrt()) + 1e-6))
+        check_step(opt, params, Oracle(), counts, bits, k)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_parameters_without_a_gradient_keep_their_own_count(bits):
     import myria3d_amd

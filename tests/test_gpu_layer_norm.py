@@ -104,6 +104,12 @@ def test_row_counts_and_weight_types(rows, cols, dtype, wtype):
     run_case(rows, cols, dtype, wtype, seed=rows)
 
 
+@pytest.mark.parametrize("rows, cols, dtype", [(350001, 100, torch.float32), (20001, 4100, torch.bfloat16), (1500001, 33, torch.float16),
+                                               (8000, 9000, torch.float32)])
+def test_what_the_caches_do_not_hold(rows, cols, dtype):
+    run_case(rows, cols, dtype, torch.float32, slope=0.2, seed=rows)
+
+
 @pytest.mark.parametrize("pad", [1, 2, 5, 8])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_with_a_stride_of_their_own(pad, dtype):
