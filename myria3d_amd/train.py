@@ -220,6 +220,7 @@ def _types(tensors: List[Tensor], who: str) -> array:
 
 
 def _check_strided(tensors: List[Tensor]) -> None:
+    """(of tensors that are not all contiguous: a sparse one never says that it is)"""
     if any(map(_SPARSE, tensors)):
         raise RuntimeError("sparse gradients are not supported")
 
@@ -239,15 +240,17 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm must not be negative, got {max_norm}")
-    grads = [g for g in map(_GRAD, params) if g is not None]
+    grads = list(map(_GRAD, params))
+    if not all(map(is_not, grads, repeat(None))):
+        grads = [g for g in grads if g is not None]
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=params[0].device if params else "cpu")
     types = _types(grads, "clip_grad_norm_: gradients")
-    _check_strided(grads)
     if len(set(map(Tensor.get_device, grads))) > 1:
         raise ValueError("clip_grad_norm_: all gradients must be on one device")
     dense = grads
     if not all(map(Tensor.is_contiguous, grads)):
+        _check_strided(grads)
         dense = [g if _dense(g) else g.contiguous() for g in grads]
     ptrs, numel = _pointers(dense), _sizes(dense)
     if len(set(ptrs)) < len(ptrs) and len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads):
@@ -414,10 +417,10 @@ class AdamW(torch.optim.Optimizer):
         if not all(map(is_not, grads, repeat(None))):
             there = [x for x in grads if x is not None]
             numel, types = (array(a.typecode, (n for n, x in zip(a, grads) if x is not None)) for a in (numel, types))
-        _check_strided(there)
         if _sizes(there) != numel or _types(there, "AdamW: gradients") != types or not set(map(Tensor.get_device, there)) <= {self._device.index}:
             raise RuntimeError("AdamW: a gradient must have its parameter's size, type and device")
         if not (g.plain and all(map(Tensor.is_contiguous, there))):
+            _check_strided(there)
             grads = [None if x is None else _like(x, p) for x, p in zip(grads, g.params)]
             there = [x for x in grads if x is not None]
         if len(there) == len(grads):
@@ -497,6 +500,8 @@ class AdamW(torch.optim.Optimizer):
             for p, e in zip(g.params, entries):
                 if e and tuple(e["exp_avg"].shape) != tuple(p.shape):
                     raise ValueError(f"optimizer state has shape {tuple(e['exp_avg'].shape)}, expected {tuple(p.shape)}")
+                if e and "exp_avg_scale" in e and not (e["exp_avg"].is_contiguous() and p.is_contiguous()) and e["exp_avg"].stride() != p.stride():
+                    raise ValueError("8-bit states belong to the memory order of the parameter that they were saved from")
             if len(coded) > 1 or (True in coded and g.bits != 8):
                 raise ValueError("8-bit states go into an optimizer with state_bits=8 only")
             todo.append((g, group, entries, True in coded))
@@ -522,5 +527,10 @@ class AdamW(torch.optim.Optimizer):
             g.state[0] = top
             g.missed.copy_(torch.tensor([int(top - s) for s in steps], dtype=torch.int32))
             for k, v in group.items():
-                if k != "params" and k in mine:
-                    mine[k] = v
+                if k == "lr" and isinstance(mine["lr"], Tensor):
+                    mine["lr"].fill_(float(v))  # (the place that a captured step reads)
+                elif k != "params" and k in mine:
+                    mine[k] = float(v) if isinstance(v, Tensor) else v
+
+    def __getstate__(self):
+        raise TypeError("AdamW cannot be copied or pickled: make another one and load state_dict()")

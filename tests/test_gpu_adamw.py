@@ -442,6 +442,24 @@ def test_state_dict_continues_the_run(bits):
             myria3d_amd.AdamW(twins).load_state_dict(saved)
     with pytest.raises(ValueError):
         myria3d_amd.AdamW(twins[:3], state_bits=bits).load_state_dict(saved)
+    with pytest.raises(TypeError):
+        copy.deepcopy(opt)
+    lr = torch.tensor(0.5, device="cuda")
+    there = myria3d_amd.AdamW(twins, lr=lr, state_bits=bits)
+    there.load_state_dict(saved)
+    assert there.param_groups[0]["lr"] is lr and float(lr) == pytest.approx(1e-2)
+    a = torch.zeros(30, 40, device="cuda").requires_grad_()
+    b = torch.zeros(40, 30, device="cuda").t().requires_grad_()
+    a.grad = torch.randn(30, 40, device="cuda")
+    first = myria3d_amd.AdamW([a], state_bits=bits)
+    first.step()
+    if bits == 8:  # (blocks run along memory)
+        with pytest.raises(ValueError):
+            myria3d_amd.AdamW([b], state_bits=8).load_state_dict(first.state_dict())
+    else:
+        second = myria3d_amd.AdamW([b])
+        second.load_state_dict(first.state_dict())
+        assert torch.equal(moments_of(second)[0][0], moments_of(first)[0][0])
 
 
 def test_states_travel_to_and_from_torch():
@@ -502,6 +520,25 @@ def test_replayed_steps_count_on(bits):
     side.synchronize()
     ref.step()
     assert all(torch.equal(p, q) for p, q in zip(params, twins))
+
+
+def test_parameters_that_move_and_change():
+    import myria3d_amd
+
+    for change, fails in ((lambda p: p.data.clone(), False), (lambda p: p.data.cpu(), True), (lambda p: p.data.double(), True),
+                          (lambda p: p.data.t().contiguous().t(), True), (lambda p: torch.zeros(5, 7, device="cuda"), True)):
+        p = torch.randn(6, 8, device="cuda", requires_grad=True)
+        p.grad = torch.randn(6, 8, device="cuda")
+        opt = myria3d_amd.AdamW([p])
+        check_step(opt, [p], Oracle(), [0], 32)
+        g, p.grad = p.grad, None
+        p.data = change(p)
+        if fails:
+            with pytest.raises((RuntimeError, TypeError)):
+                opt.step()
+        else:
+            p.grad = g
+            check_step(opt, [p], Oracle(), [1], 32)
 
 
 def test_version_counters_and_exchanged_parameters():
