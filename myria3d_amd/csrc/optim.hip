@@ -9,8 +9,8 @@
 // memory bounds all of it and the design is about few launches and few bytes:
 //   * the tensors' pointers travel as KERNEL ARGUMENTS (up to OPT_TENSORS a launch): no table in device memory to upload when a
 //     gradient moves, nothing to keep alive, and a captured graph holds its own copy;
-//   * a tensor is cut into blocks of 256 elements, numbered through over all tensors; a workgroup takes a contiguous run of
-//     blocks and finds its first tensor by a binary search over the arguments (scalar loads).  The moments live in flat buffers in
+//   * a tensor is cut into blocks of 256 elements, numbered through over all tensors; workgroups take runs of up to 32 blocks in
+//     turn and find a run's first tensor by a binary search over the arguments (scalar loads).  The moments live in flat buffers in
 //     the same numbering (every tensor's slice starts at a multiple of 256);
 //   * the norm is two steps without a launch of its own in between: workgroups leave fp64 partial sums, and whoever needs the
 //     norm (the clip kernel, the AdamW kernel) adds them up, in a fixed order, at its start;
@@ -734,12 +734,15 @@ extern "C" int m3d_adamw_step(const M3DAdamW* a, void* stream) {
   if ((((uintptr_t)a->exp_avg) | ((uintptr_t)a->exp_avg_sq)) & 15) return M3D_ERR_INVALID;
   for (int32_t i = 0; i < a->count; ++i)
     if (a->numel[i] > 0 && !a->params[i]) return M3D_ERR_INVALID;
+  if (!(a->eps >= 0.0) || (a->state_bits == 8 && a->eps == 0.0)) return M3D_ERR_INVALID;
   if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0)) return M3D_ERR_INVALID;
   if (a->parts && (a->nparts < 1 || a->nparts > OPT_PARTS || !(a->max_norm >= 0.0))) return M3D_ERR_INVALID;
   AdamArgs A{};
   A.m = a->exp_avg; A.v = a->exp_avg_sq; A.ms = a->scale_avg; A.vs = a->scale_avg_sq;
   A.state = a->state; A.missed = a->missed; A.parts = a->parts; A.nparts = a->nparts; A.lr_dev = a->lr_dev;
-  A.max_norm = a->max_norm; A.lr = a->lr; A.wd = a->weight_decay; A.eps = (float)a->eps;
+  A.max_norm = a->max_norm; A.lr = a->lr; A.wd = a->weight_decay;
+  // (the reciprocal instruction takes what is under 2^-126 for zero; an eps of zero stays one, as in the formula)
+  A.eps = a->eps > 0.0 && a->eps < 0x1p-126 ? 0x1p-126f : (float)a->eps;
   A.b1 = a->beta1; A.b2 = a->beta2; A.c1 = 1.0 - a->beta1; A.c2 = 1.0 - a->beta2;
   A.log_b1 = log(a->beta1); A.log_b2 = log(a->beta2);
   double bytes = 0.0;

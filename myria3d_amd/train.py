@@ -358,12 +358,11 @@ class AdamW(torch.optim.Optimizer):
             self.grad_norm = torch.zeros((), dtype=torch.float32, device=self._device)
             self._parts = torch.empty(GRAD_NORM_PARTS, dtype=torch.float64, device=self._device)
 
-    @staticmethod
-    def _check_group(g: dict, bits: int) -> None:
-        lr, (b1, b2), eps, wd = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+    def _check_group(self, g: dict) -> None:
+        lr, (b1, b2), eps, wd, bits = g["lr"], g["betas"], g["eps"], g["weight_decay"], self.state_bits
         if isinstance(lr, Tensor):
-            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
-                raise ValueError("AdamW: a tensor lr must be one fp32 element on the device")
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda or (self._device is not None and lr.device != self._device):
+                raise ValueError("AdamW: a tensor lr must be one fp32 element on the parameters' device")
         elif not (float(lr) >= 0.0 and math.isfinite(lr)):
             raise ValueError(f"AdamW: lr must not be negative, got {lr}")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
@@ -380,10 +379,12 @@ class AdamW(torch.optim.Optimizer):
             params = group["params"]
             if not params:
                 raise ValueError("AdamW: a parameter group without parameters")
-            self._check_group(group, self.state_bits)
+            self._check_group(group)
             if len({id(p) for p in params}) < len(params):
                 raise ValueError("AdamW: the same parameter twice in a group")
             dev = self._device or params[0].device
+            if isinstance(group["lr"], Tensor) and group["lr"].device != dev:
+                raise ValueError("AdamW: a tensor lr must be one fp32 element on the parameters' device")
             for p in params:
                 if p.dtype not in ops.TYPES:
                     raise TypeError(f"AdamW: parameters must be float32, bfloat16 or float16, got {p.dtype}")
@@ -435,7 +436,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         pointers, keep = [], []
         for g, group in zip(self._groups, self.param_groups):
-            self._check_group(group, self.state_bits)
+            self._check_group(group)
             if len(group["params"]) != len(g.params) or not all(map(is_, group["params"], g.params)):
                 raise RuntimeError("AdamW: the parameters of a group were exchanged after the optimizer was made")
             params = self._parameters(g)

@@ -522,6 +522,19 @@ def test_replayed_steps_count_on(bits):
     assert all(torch.equal(p, q) for p, q in zip(params, twins))
 
 
+def test_an_eps_under_the_smallest_normal_number_leaves_dead_elements_alone():
+    import myria3d_amd
+
+    for bits in (32, 8):
+        p = torch.ones(600, device="cuda", requires_grad=True)
+        p.grad = torch.zeros(600, device="cuda")
+        p.grad[:5] = 1.0
+        opt = myria3d_amd.AdamW([p], lr=0.25, eps=1e-42, weight_decay=0.0, state_bits=bits)
+        opt.step()
+        # the update of a first step is lr against the sign: 14 roundings of a quarter
+        assert bool((p[5:] == 1.0).all()) and bool(((p[:5] - 0.75).abs() <= 14 * U).all())
+
+
 def test_parameters_that_move_and_change():
     import myria3d_amd
 

@@ -138,7 +138,8 @@ def test_many_tensor_entry_points_refuse():
     assert h.m3d_adamw_step(None, None) == -1
     keep3, (none, _, _) = _arrays([0], [4], [0])
     for kw in ({"params": none}, {"exp_avg": None}, {"exp_avg_sq": P + 4}, {"state": None}, {"missed": None}, {"beta1": 1.0}, {"beta2": -0.5},
-               {"state_bits": 8, "scale_avg": None}, {"parts": P, "nparts": 0}, {"parts": P, "nparts": 4, "max_norm": -1.0}):
+               {"state_bits": 8, "scale_avg": None}, {"parts": P, "nparts": 0}, {"parts": P, "nparts": 4, "max_norm": -1.0},
+               {"eps": -1.0}, {"eps": float("nan")}, {"state_bits": 8, "eps": 0.0}):
         assert step(**kw) == -1, kw
     assert step(state_bits=16) == -2
     assert h.m3d_moments_decode(None, P, P, P, P, P, 1, None) == -1 and h.m3d_moments_decode(P, P, P, P, P, P + 4, 1, None) == -1
