@@ -201,11 +201,11 @@ _GRAD, _DTYPE, _SPARSE = attrgetter("grad"), attrgetter("dtype"), attrgetter("is
 
 
 def _pointers(tensors: List[Tensor]) -> array:
-    return array("Q", map(Tensor.data_ptr, tensors))
+    return array("Q", list(map(Tensor.data_ptr, tensors)))  # (an array grows element by element from anything but a list)
 
 
 def _sizes(tensors: List[Tensor]) -> array:
-    return array("q", map(Tensor.numel, tensors))
+    return array("q", list(map(Tensor.numel, tensors)))
 
 
 def _types(tensors: List[Tensor], who: str) -> array:

@@ -522,6 +522,58 @@ def test_replayed_steps_count_on(bits):
     assert all(torch.equal(p, q) for p, q in zip(params, twins))
 
 
+def test_clipping_in_a_graph():
+    import myria3d_amd
+
+    params = tensors(SIZES * 20, DTYPES, 15)
+    myria3d_amd.clip_grad_norm_(params, 1e9)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = myria3d_amd.clip_grad_norm_(params, 2.0)
+    for k in range(4):
+        for p in params:
+            p.grad.copy_(torch.randn(p.shape, device="cuda"))
+        twins = [p.detach().clone().requires_grad_() for p in params]
+        for p, q in zip(params, twins):
+            q.grad = p.grad.clone()
+        want = myria3d_amd.clip_grad_norm_(twins, 2.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want) and all(torch.equal(p.grad, q.grad) for p, q in zip(params, twins)), k
+
+
+def test_closures_schedules_scalars_and_groups_that_come_later():
+    import myria3d_amd
+
+    a = torch.tensor(2.0, device="cuda", requires_grad=True)  # no dimension
+    e = torch.zeros(0, 3, device="cuda", requires_grad=True)  # no element
+    opt = myria3d_amd.AdamW([a, e], lr=0.1, weight_decay=0.0)
+    late = torch.ones(300, device="cuda", requires_grad=True)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+
+    def closure():
+        opt.zero_grad()
+        loss = a * a + late.sum() + e.sum()
+        loss.backward()
+        return loss
+
+    assert float(opt.step(closure)) == 304.0
+    sched.step()
+    assert abs(float(a) - 1.9) <= 16 * U * 2 and not late.ne(1.0).any()  # a first step is lr against the sign
+    opt.add_param_group({"params": [late], "lr": 0.25})
+    opt.step(closure)
+    assert bool(((late - 0.75).abs() <= 16 * U).all())  # its own count: a first step
+    assert [int(s["step"]) for s in opt.state_dict()["state"].values()] == [2, 2, 1]
+    assert [g["lr"] for g in opt.param_groups] == [0.05, 0.25]
+    only = myria3d_amd.AdamW([e], state_bits=8, max_grad_norm=1.0)
+    only.step()
+    assert float(only.grad_norm) == 0.0 and only.moments()[0][0].numel() == 0
+    only.load_state_dict(only.state_dict())
+    named = myria3d_amd.AdamW(torch.nn.Linear(3, 2, device="cuda").named_parameters())
+    named.step()  # no gradient anywhere: nothing happens
+    assert {float(s["step"]) for s in named.state_dict()["state"].values()} == {0.0}
+
+
 def test_an_eps_under_the_smallest_normal_number_leaves_dead_elements_alone():
     import myria3d_amd
 

@@ -230,6 +230,20 @@ def test_only_the_gradients_that_are_asked_for():
             assert torch.equal(one, every[k])
 
 
+def test_a_second_derivative_is_refused_and_inference_runs():
+    import myria3d_amd
+
+    x, w = torch.randn(4, 16, device="cuda", requires_grad=True), torch.randn(16, device="cuda", requires_grad=True)
+    y = myria3d_amd.layer_norm(x, w)
+    (plain,) = torch.autograd.grad(y.square().sum(), x, retain_graph=True)
+    (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), x)
+    with torch.inference_mode():
+        assert torch.equal(myria3d_amd.layer_norm(x, w), y.detach())
+
+
 def test_offsets_beyond_32_bits():
     import myria3d_amd
 
