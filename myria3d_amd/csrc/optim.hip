@@ -264,12 +264,15 @@ __device__ __forceinline__ AdamStep adam_step_of(const AdamArgs& A, double t, do
 // than the codes do).
 #define NAN_M 0x7fu
 #define NAN_V 0xffu
-__device__ __forceinline__ int sticky_word(double x) { return __double2hiint(x) | (__double2loint(x) != 0 ? 1 : 0); }
+__device__ __forceinline__ int sticky_word(double x) {
+  const uint32_t lo = (uint32_t)__double2loint(x);
+  return __double2hiint(x) | (int)(lo < 1u ? lo : 1u);  // (one minimum: the compiler's own form of lo != 0 is a comparison and a select)
+}
 // decoded, as held: one rounding in 32 bits (the factor 2^-8 is exact: the block's largest magnitude has code 256)
 __device__ __forceinline__ void decode_m4(uint32_t c, float s, float (&m)[4]) {
-  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-  const float k = 0.00390625f;
-  m[0] = a[0] * k * s; m[1] = a[1] * k * s; m[2] = b[0] * k * s; m[3] = b[1] * k * s;
+  const float k = 0.00390625f;  // (the conversion scales by powers of two)
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, k, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, k, true);
+  m[0] = a[0] * s; m[1] = a[1] * s; m[2] = b[0] * s; m[3] = b[1] * s;
 }
 // u(c) = 2^((c >> 3) - 31) (1 + (c & 7) / 8): the code is the upper part of a float with its exponent moved
 __device__ __forceinline__ void decode_v4(uint32_t q, float s, float (&v)[4]) {
@@ -307,7 +310,7 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     mx = umax(mx, __float_as_uint(mf[j]) & 0x7fffffffu);
-    vx = umax(vx, __float_as_uint(vf[j]) & 0x7fffffffu);
+    vx = umax(vx, __float_as_uint(vf[j]));  // (with its sign: what is negative here is no second moment, and counts as not finite)
   }
   mx = wave_umax(mx);
   vx = wave_umax(vx);
@@ -317,7 +320,7 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
     mx = vx = 0u;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t a = __float_as_uint(mf[j]) & 0x7fffffffu, b = __float_as_uint(vf[j]) & 0x7fffffffu;
+      const uint32_t a = __float_as_uint(mf[j]) & 0x7fffffffu, b = __float_as_uint(vf[j]);
       mx = umax(mx, a < inf ? a : 0u);
       vx = umax(vx, b < inf ? b : 0u);
     }
@@ -355,7 +358,8 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
     r[j] = (float)__hiloint2double(sticky_word(qm[j]), 0);  // (exact; the conversion below rounds to nearest even)
     const uint32_t u = (uint32_t)sticky_word(qv[j]);
     const int k = (int)((u + 0xffffu + ((u >> 17) & 1u)) >> 17) - ((1023 - 31) << 3);  // nearest even at three bits of fraction
-    c[j] = u ? (uint32_t)(k < 1 ? 1 : k) : 0u;                                         // what is above zero stays above it
+    const int least = (int)(u < 1u ? u : 1u);  // what is above zero stays above it
+    c[j] = (uint32_t)(k < least ? least : k);
   }
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], w, true);
@@ -365,7 +369,7 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if ((__float_as_uint(mf[j]) & 0x7fffffffu) >= inf) cm = (cm & ~(0xffu << (8 * j))) | (NAN_M << (8 * j));
-      if ((__float_as_uint(vf[j]) & 0x7fffffffu) >= inf) c[j] = NAN_V;  // (the others are 248 at most)
+      if (__float_as_uint(vf[j]) >= inf) c[j] = NAN_V;  // (the others are 248 at most)
     }
   }
   cv = c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24);
@@ -373,10 +377,20 @@ __device__ __forceinline__ void encode_block(const double (&m)[4], const double 
 
 // sqrt and quotient by the instructions (each within one unit in the last place; the update is a small part of the parameter):
 // what the compiler makes of sqrtf and / costs 25 instructions an element.  The square root's argument is kept out of the denormals.
-__device__ __forceinline__ float quick_sqrt(float v) {
-  const bool tiny = v < 0x1p-96f;
-  const float r = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v);
-  return tiny ? r * 0x1p-32f : r;
+// Beside an eps of 2^-40 or more the root of a denormal number, under 2^-63, says nothing, whatever the instruction makes of it.
+__device__ __forceinline__ void quick_roots(const float (&v)[4], float eps, float (&r)[4]) {
+  if (eps >= 0x1p-40f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_sqrtf(v[j]);
+  } else {
+    asm volatile("" ::: );  // (a branch)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool tiny = v[j] < 0x1p-96f;
+      const float t = __builtin_amdgcn_sqrtf(tiny ? v[j] * 0x1p64f : v[j]);
+      r[j] = tiny ? t * 0x1p-32f : t;
+    }
+  }
 }
 
 // a lane's four elements as they lie in memory
@@ -425,9 +439,9 @@ __device__ __forceinline__ void raw_values(const Raw& r, int type, float (&v)[4]
 // (with single blocks dealt out to the waves of all workgroups: 590 against 440 us for 100 M parameters with 8-bit moments).
 //   32 bits: bound by memory.  The next block is on its way while the present one is computed.  75 M bf16 parameters (22 bytes each):
 //     270 us, 6.1 TB/s, what a large scaling reaches here; 3 M fp32 (28 bytes): 19.5 us.
-//   8 bits: 85 vector instructions an element, a third of them in 64 bits (whose rate is that of 32), beside 16 bytes: 100 M fp32
-//     parameters take 350 us, 4.6 TB/s, of which the instructions alone are about 220.  Fetching ahead costs more in registers than it
-//     hides (385 us).
+//   8 bits: 85 vector instructions an element, a third of them in 64 bits, beside 16 bytes: the vector units are busy 71 % of the
+//     time (SQ counters) and 100 M fp32 parameters take 350 us, 4.6 TB/s.  Six or seven waves on a SIMD instead of five change
+//     nothing; fetching ahead costs more in registers than it hides (389 us).
 // ONCE: past the caches (see M3D_CACHE_BYTES), but for what is written of the parameters, which the forward pass reads next.
 template <int BITS, bool ONCE>
 __global__ __launch_bounds__(256, 5) void adamw_kernel(const TensorList L, const AdamArgs A) {
@@ -556,8 +570,10 @@ __global__ __launch_bounds__(256, 5) void adamw_kernel(const TensorList L, const
           ((uint32_t*)A.v)[s] = cv;
           if (lane == 0) { A.ms[cur.b] = nm; A.vs[cur.b] = nv; }
         }
+        float root[4];
+        quick_roots(vf, A.eps, root);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = p[j] * S.decay - S.size * mf[j] * __builtin_amdgcn_rcpf(quick_sqrt(vf[j]) * S.root + A.eps);
+        for (int j = 0; j < 4; ++j) p[j] = p[j] * S.decay - S.size * mf[j] * __builtin_amdgcn_rcpf(root[j] * S.root + A.eps);
         if (cur.n > 0) store4(L.p[cur.t], cur.e, cur.n, cur.type, p);
       }
       if (!more) break;
