@@ -401,10 +401,10 @@ class AdamW(torch.optim.Optimizer):
     # ------------------------------------------------------------------------------------------
     def _parameters(self, g: _Group) -> array:
         """Pointers of a group's parameters.  The aliases made with the group keep the memory that they were found in alive: where the
-        pointers are the same, the parameters are where they were; elsewhere everything about them is looked at again."""
-        ptrs = _pointers(g.params)
-        if ptrs != g.pointers:
-            params = g.params
+        pointers (and the order) are the same, the parameters are where they were; elsewhere everything about them is looked at again."""
+        params = g.params
+        ptrs = _pointers(params)
+        if ptrs != g.pointers or not (all(map(Tensor.is_contiguous, params)) if g.plain else [p.stride() for p in params] == g.strides):
             if (_sizes(params) != g.numel or _types(params, "AdamW: parameters") != g.types or [p.stride() for p in params] != g.strides
                     or {p.get_device() for p in params} != {self._device.index}):
                 raise RuntimeError("AdamW: a parameter changed its size, type, order or device after the optimizer was made")

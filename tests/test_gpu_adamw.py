@@ -591,7 +591,7 @@ def test_parameters_that_move_and_change():
     import myria3d_amd
 
     for change, fails in ((lambda p: p.data.clone(), False), (lambda p: p.data.cpu(), True), (lambda p: p.data.double(), True),
-                          (lambda p: p.data.t().contiguous().t(), True), (lambda p: torch.zeros(5, 7, device="cuda"), True)):
+                          (lambda p: p.data.t().contiguous().t(), True), (lambda p: p.data.t(), True), (lambda p: torch.zeros(5, 7, device="cuda"), True)):
         p = torch.randn(6, 8, device="cuda", requires_grad=True)
         p.grad = torch.randn(6, 8, device="cuda")
         opt = myria3d_amd.AdamW([p])
