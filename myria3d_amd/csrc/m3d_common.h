@@ -11,8 +11,9 @@
 
 #define M3D_WAVE 64
 
-// the cache in front of the memory.  A kernel whose call touches more than this once loads and stores past it (nontemporal): the lines
-// would be gone before anyone came back for them, and their write-backs cost the kernels behind
+// The cache in front of the memory.  A kernel whose call touches more than this loads and stores past it (nontemporal): the lines
+// would be gone before anyone came back for them, and their write-backs cost the kernels behind.  Layer norm's backward pass, 1.6 M x 64
+// fp32: 241 -> 203 us, AdamW over 75 M parameters: 336 -> 270 us; inside the cache it loses (12 801 x 515 fp16: 14 -> 16 us).
 #ifndef M3D_CACHE_BYTES
 #define M3D_CACHE_BYTES (256ll << 20)
 #endif

@@ -22,7 +22,7 @@
 #define OPT_TENSORS 152   // 24 bytes each: the list stays under 4 KB of kernel arguments (HipRandLANet has 141 tensors: one launch)
 #define OPT_BLOCK 256     // elements of a block (and of one 8-bit scale)
 #define OPT_PARTS M3D_GRAD_NORM_PARTS
-#define OPT_CHUNK 32      // blocks a workgroup takes at a time where there are many: 16 or 32 KB, one run of memory
+#define OPT_CHUNK 32      // blocks a workgroup takes at a time where there are many: 16 or 32 KB, one run of memory (AdamW, 75 M: 270 us; 64: 290)
 #define OPT_DECODE 4      // blocks a wave decodes side by side
 
 struct TensorList {
@@ -437,8 +437,8 @@ __device__ __forceinline__ void raw_values(const Raw& r, int type, float (&v)[4]
 // A workgroup walks chunks of up to 32 blocks, its four waves take a chunk's blocks in turn, a lane four consecutive elements (16-byte
 // accesses in fp32); all workgroups together walk one window of memory, and a chunk's 8-bit scales, one line of cache, have one writer
 // (with single blocks dealt out to the waves of all workgroups: 590 against 440 us for 100 M parameters with 8-bit moments).
-//   32 bits: bound by memory.  The next block is on its way while the present one is computed.  75 M bf16 parameters (22 bytes each):
-//     270 us, 6.1 TB/s, what a large scaling reaches here; 3 M fp32 (28 bytes): 19.5 us.
+//   32 bits: bound by memory.  The next block is on its way while the present one is computed (320 us without).  75 M bf16 parameters
+//     (22 bytes each): 270 us, 6.1 TB/s, what a large scaling reaches here; 3 M fp32 (28 bytes): 19.5 us.
 //   8 bits: 85 vector instructions an element, a third of them in 64 bits, beside 16 bytes: the vector units are busy 71 % of the
 //     time (SQ counters) and 100 M fp32 parameters take 350 us, 4.6 TB/s.  Six or seven waves on a SIMD instead of five change
 //     nothing; fetching ahead costs more in registers than it hides (389 us).
@@ -589,10 +589,10 @@ __global__ __launch_bounds__(256, 5) void adamw_kernel(const TensorList L, const
   __syncthreads();  // every thread of this workgroup has used its copy of the count
   if (threadIdx.x == 0) {  // two levels of tickets: one address takes ~15 ns an arrival
     unsigned* tk = (unsigned*)&A.state[1];
-    const unsigned subs = gridDim.x <= 256 ? 16 : 64, sub = blockIdx.x % subs, members = gridDim.x / subs + (sub < gridDim.x % subs ? 1u : 0u);
+    const unsigned sub = blockIdx.x % 64, members = gridDim.x / 64 + (sub < gridDim.x % 64 ? 1u : 0u);
     if (atomicAdd(&tk[1 + sub], 1u) == members - 1) {
       tk[1 + sub] = 0u;
-      const unsigned groups = gridDim.x < subs ? gridDim.x : subs;
+      const unsigned groups = gridDim.x < 64 ? gridDim.x : 64;
       if (atomicAdd(&tk[0], 1u) == groups - 1) {
         if (go) __hip_atomic_store(&A.state[0], (float)(done + 1.0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         tk[0] = 0u;
@@ -601,7 +601,8 @@ __global__ __launch_bounds__(256, 5) void adamw_kernel(const TensorList L, const
   }
 }
 
-// ---- 8-bit moments <-> 32 bits (checkpoints, inspection)
+// ---- 8-bit moments <-> 32 bits (checkpoints, inspection).  200 M elements decoded: 361 us, 5.5 TB/s, mostly writes (383 with 2 048
+// workgroups that go on, 424 with one block a wave at a time).
 __global__ __launch_bounds__(256) void moments_decode_kernel(const uint32_t* __restrict__ qm, const uint32_t* __restrict__ qv,
                                                              const float* __restrict__ sm, const float* __restrict__ sv,
                                                              f32x4* __restrict__ m, f32x4* __restrict__ v, int64_t blocks) {
