@@ -271,9 +271,18 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   const int64_t step = (int64_t)gridDim.x * per;
   int64_t row = (int64_t)blockIdx.x * per + (IN ? threadIdx.x / G : 0);
   const int64_t turns = (A.rows - (int64_t)blockIdx.x * per + step - 1) / step;
-  Raw<NE> nx = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
-  Raw<NE> ng = raw_load<TYPE, NE, ONCE>(A.dy, row * A.lddy, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
-  float nmean = row < A.rows ? A.mean[row] : 0.f, nrstd = row < A.rows ? A.rstd[row] : 0.f;
+  // (1 024 threads with 16 elements each have no registers for a row ahead: 6 000 x 8 199 fp32, both passes, 525 us with, 247 without)
+  constexpr bool AHEAD = TPR != 1024 || NE * V < 16;
+  Raw<NE> nx, ng;
+  float nmean, nrstd;
+  auto fetch = [&](int64_t r) {
+    const bool there = r < A.rows;
+    nx = raw_load<TYPE, NE, ONCE>(A.x, r * A.ldx, lane, lanes, there ? nv : 0, rest, there && has_rest);
+    ng = raw_load<TYPE, NE, ONCE>(A.dy, r * A.lddy, lane, lanes, there ? nv : 0, rest, there && has_rest);
+    nmean = there ? A.mean[r] : 0.f;
+    nrstd = there ? A.rstd[r] : 0.f;
+  };
+  if constexpr (AHEAD) fetch(row);
   w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
   if constexpr (ACT) w_loads<V, NE>(A.b, A.wtype, 0.f, lane, lanes, nv, rest, has_rest, b);
 #pragma unroll
@@ -281,17 +290,12 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   int flip = 0;
   for (int64_t turn = 0; turn < turns; ++turn, row += step) {
     const bool on = row < A.rows;
+    if constexpr (!AHEAD) fetch(row);
     float x[E], g[E];
     raw_values<TYPE, NE>(nx, x);
     raw_values<TYPE, NE>(ng, g);
     const float mean = nmean, rstd = nrstd;
-    {
-      const bool more = row + step < A.rows;
-      nx = raw_load<TYPE, NE, ONCE>(A.x, (row + step) * A.ldx, lane, lanes, more ? nv : 0, rest, more && has_rest);
-      ng = raw_load<TYPE, NE, ONCE>(A.dy, (row + step) * A.lddy, lane, lanes, more ? nv : 0, rest, more && has_rest);
-      nmean = more ? A.mean[row + step] : 0.f;
-      nrstd = more ? A.rstd[row + step] : 0.f;
-    }
+    if constexpr (AHEAD) fetch(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -486,9 +490,12 @@ static NormShape norm_shape(int32_t cols, int32_t type, bool bwd) {
 static int norm_per(const NormShape& s) { return s.tpr && s.tpr <= 64 ? 256 / s.tpr : 1; }
 // Workgroups: at most 16 waves on each of the 256 compute units (8 in the backward pass with several rows a wave, whose registers
 // allow little more and whose ends, w, b, dw and db, cost more than they hide: 241 against 259 us at 1.6 M x 64 fp32), each with
-// the same number of turns.
-static int64_t norm_grid(const NormShape& s, int64_t rows, bool bwd) {
-  const int64_t most = 256 * (bwd && s.threads == 256 && norm_per(s) > 1 ? 2 : 1024 / s.threads), need = m3d_cdiv(rows, norm_per(s));
+// the same number of turns.  Rows of up to 40 bytes: what the registers allow, since only many waves keep some of them in flight (20 M x 3
+// fp32, both passes: 882 -> 555 us, 12 M x 7: 661 -> 533; but 6 M x 15: 450 -> 556).
+static int64_t norm_grid(const NormShape& s, int64_t rows, int32_t cols, int32_t type, bool bwd) {
+  const bool few = cols <= (type == M3D_TYPE_F32 ? 10 : 20);
+  const int per_unit = few ? (bwd ? 5 : 8) : bwd && s.threads == 256 && norm_per(s) > 1 ? 2 : 1024 / s.threads;
+  const int64_t most = 256 * per_unit, need = m3d_cdiv(rows, norm_per(s));
   return need <= most ? need : m3d_cdiv(need, m3d_cdiv(need, most));
 }
 static bool norm_once(int64_t rows, int32_t cols, int32_t type, int matrices) {
@@ -562,12 +569,12 @@ extern "C" int m3d_layer_norm_fwd(const void* x, int64_t ldx, const void* w, con
   A.x = x; A.w = w; A.b = b; A.y = y; A.mean = mean; A.rstd = rstd; A.rows = rows; A.ldx = ldx; A.cols = cols; A.wtype = wtype;
   A.eps = eps; A.slope = slope; A.inv = 1.f / (float)cols;
   const NormShape s = norm_shape(cols, type, false);
-  return launch_norm_any(A, s, norm_grid(s, rows, false), type, false, (hipStream_t)stream);
+  return launch_norm_any(A, s, norm_grid(s, rows, cols, type, false), type, false, (hipStream_t)stream);
 }
 
 extern "C" size_t m3d_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t type) {
   if (rows <= 0 || cols < 1 || !norm_type_ok(type)) return 0;
-  return (size_t)norm_grid(norm_shape(cols, type, true), rows, true) * 2 * (size_t)cols * sizeof(float);
+  return (size_t)norm_grid(norm_shape(cols, type, true), rows, cols, type, true) * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const void* b, const float* mean,
@@ -585,7 +592,7 @@ extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, i
   A.cols = cols; A.wtype = wtype; A.slope = slope; A.inv = 1.f / (float)cols;
   A.parts = (dw || db) ? (float*)ws : nullptr;
   const NormShape s = norm_shape(cols, type, true);
-  const int64_t grid = norm_grid(s, rows, true);
+  const int64_t grid = norm_grid(s, rows, cols, type, true);
   if (rows > 0 && (dx || A.parts)) {
     const int rc = launch_norm_any(A, s, grid, type, true, st);
     if (rc != M3D_OK) return rc;
