@@ -271,18 +271,16 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   const int64_t step = (int64_t)gridDim.x * per;
   int64_t row = (int64_t)blockIdx.x * per + (IN ? threadIdx.x / G : 0);
   const int64_t turns = (A.rows - (int64_t)blockIdx.x * per + step - 1) / step;
-  // (1 024 threads with 16 elements each have no registers for a row ahead: 6 000 x 8 199 fp32, both passes, 525 us with, 247 without)
+  // (1 024 threads with 16 elements each have no registers for a row ahead: 6 000 x 8 199 fp32, both passes, 510 us with, 235 without)
   constexpr bool AHEAD = TPR != 1024 || NE * V < 16;
   Raw<NE> nx, ng;
-  float nmean, nrstd;
-  auto fetch = [&](int64_t r) {
-    const bool there = r < A.rows;
-    nx = raw_load<TYPE, NE, ONCE>(A.x, r * A.ldx, lane, lanes, there ? nv : 0, rest, there && has_rest);
-    ng = raw_load<TYPE, NE, ONCE>(A.dy, r * A.lddy, lane, lanes, there ? nv : 0, rest, there && has_rest);
-    nmean = there ? A.mean[r] : 0.f;
-    nrstd = there ? A.rstd[r] : 0.f;
-  };
-  if constexpr (AHEAD) fetch(row);
+  float nmean = 0.f, nrstd = 0.f;
+  if constexpr (AHEAD) {
+    nx = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
+    ng = raw_load<TYPE, NE, ONCE>(A.dy, row * A.lddy, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
+    nmean = row < A.rows ? A.mean[row] : 0.f;
+    nrstd = row < A.rows ? A.rstd[row] : 0.f;
+  }
   w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
   if constexpr (ACT) w_loads<V, NE>(A.b, A.wtype, 0.f, lane, lanes, nv, rest, has_rest, b);
 #pragma unroll
@@ -290,12 +288,23 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   int flip = 0;
   for (int64_t turn = 0; turn < turns; ++turn, row += step) {
     const bool on = row < A.rows;
-    if constexpr (!AHEAD) fetch(row);
+    if constexpr (!AHEAD) {
+      nx = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, on ? nv : 0, rest, on && has_rest);
+      ng = raw_load<TYPE, NE, ONCE>(A.dy, row * A.lddy, lane, lanes, on ? nv : 0, rest, on && has_rest);
+      nmean = on ? A.mean[row] : 0.f;
+      nrstd = on ? A.rstd[row] : 0.f;
+    }
     float x[E], g[E];
     raw_values<TYPE, NE>(nx, x);
     raw_values<TYPE, NE>(ng, g);
     const float mean = nmean, rstd = nrstd;
-    if constexpr (AHEAD) fetch(row + step);
+    if constexpr (AHEAD) {
+      const bool more = row + step < A.rows;
+      nx = raw_load<TYPE, NE, ONCE>(A.x, (row + step) * A.ldx, lane, lanes, more ? nv : 0, rest, more && has_rest);
+      ng = raw_load<TYPE, NE, ONCE>(A.dy, (row + step) * A.lddy, lane, lanes, more ? nv : 0, rest, more && has_rest);
+      nmean = more ? A.mean[row + step] : 0.f;
+      nrstd = more ? A.rstd[row + step] : 0.f;
+    }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
