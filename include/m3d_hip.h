@@ -59,7 +59,7 @@ typedef struct { const int64_t* counter; uint64_t seed; float p; const int32_t* 
 #define M3D_IO_A32 0x2000
 #define M3D_IO_C32 0x4000
 
-#define M3D_ABI_VERSION 19
+#define M3D_ABI_VERSION 20
 /* element types of the entry points that take one (M3D_TYPE_*) */
 #define M3D_TYPE_F32 0
 #define M3D_TYPE_BF16 1
@@ -524,8 +524,9 @@ int m3d_zero_bump(void* buf, int64_t nbytes, int64_t* counters, int32_t ncounter
  * (pyg_randla_net.py:92-109 has batch norm there; PyG's MLP takes norm="layer_norm"):
  *   mean, var over the row;  z = (x - mean) / sqrt(var + eps) * w + b;  y = z > 0 ? z : slope * z   (slope = 1: none)
  * x: [rows, cols], row stride ldx elements (0: the same row again); y contiguous; type: of x and y, wtype: of w and b
- * (nullable: ones, zeros).  mean, rstd: fp32 [rows] kept for the backward pass (both or neither).  Any cols >= 1; up to
- * 16 384 a row is read once. */
+ * (nullable: ones, zeros).  mean: fp32 [rows][2], a row's mean as the sum of two floats (one alone has too few digits where
+ * rows lie far from zero), rstd: fp32 [rows], kept for the backward pass (both or neither).  Any cols >= 1; up to 16 384 a
+ * row is read once. */
 int m3d_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, int64_t rows, int32_t cols, int32_t type,
                        int32_t wtype, float eps, float slope, void* y, float* mean, float* rstd, void* stream);
 size_t m3d_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t type);

@@ -133,7 +133,7 @@ class M3DAdamW(C.Structure):
                 ("eps", C.c_double), ("weight_decay", C.c_double)]
 
 
-ABI_VERSION = 19  # M3D_ABI_VERSION in include/m3d_hip.h
+ABI_VERSION = 20  # M3D_ABI_VERSION in include/m3d_hip.h
 
 _ERRORS = {-1: "invalid argument", -2: "unsupported shape", -3: "kernel launch failure"}
 

@@ -4,8 +4,14 @@
 //   g = dy (z > 0 ? 1 : slope);  dx = r (g w - mean_c(g w) - xh mean_c(g w xh));  dw = sum_rows g xh;  db = sum_rows g
 //
 // (slope = 1: no activation.)  About 8 operations an element forward and 20 backward against 4 to 12 bytes: the memory bounds
-// both, so a row is read ONCE and stays in registers — forward for the mean, the squared deviations from it (two steps: a large
-// common offset costs no digits) and the result, backward for the two row sums and the result.
+// both, so a row is read ONCE and stays in registers — forward for the mean, the squared deviations from it and the result,
+// backward for the two row sums and the result.
+//
+// The mean is held as two floats.  A first sum over cols is rounded to a float, mu1, off by its additions' roundings (3e-4 of a deviation
+// where rows lie 3 000 of them from zero, and the mean of a constant row need not be that constant).  The deviations from mu1 are
+// exact or nearly so; their own mean is what mu1 is off by, mu2.  Both sums of the second step go across the row together:
+//   sum (x - mu)^2 = sum (x - mu1)^2 - mu2 sum (x - mu1),      xh = ((x - mu1) - mu2) r
+// so a common offset costs no digits, and the backward pass, from the pair, finds the same bits of xh and the same side of the activation.
 //
 // A row belongs to TPR lanes, each with NE vectors of 16 bytes (4 fp32 or 8 half-precision elements) and, where the width is not
 // a multiple of a vector, one element of the rest.  Up to 64 lanes the row sits inside a wave (narrow rows: several rows a wave,
@@ -28,7 +34,7 @@ typedef unsigned short h4u __attribute__((ext_vector_type(4), aligned(2)));
 struct NormArgs {
   const void *x, *dy, *w, *b;
   void *y, *dx;
-  float *mean, *rstd;   // forward: written (nullable); backward: read
+  float *mean, *rstd;   // forward: written (nullable); backward: read; mean: two values a row, whose sum it is
   float* parts;         // backward: [gridDim.x][2][cols], or null: no weight gradients
   int64_t rows, ldx, lddy;
   int32_t cols, wtype;  // type of w and b
@@ -166,23 +172,41 @@ __device__ __forceinline__ float across_groups(float v) {
   return v;
 }
 // a row over a whole workgroup: wave sums through LDS; `flip` alternates the two halves of red, so that one barrier a sum is enough
-template <int S>
-__device__ __forceinline__ void wg_sums(float (&v)[S], float (*red)[16][S], int& flip) {
+template <int S, int W, typename T>
+__device__ __forceinline__ void wg_sums(T (&v)[S], T (*red)[16][W], int& flip) {
+  static_assert(S <= W, "sums of a row");
   const int waves = blockDim.x >> 6;
 #pragma unroll
-  for (int s = 0; s < S; ++s) v[s] = group_sum<64>(v[s]);
+  for (int s = 0; s < S; ++s) {
+    if constexpr (sizeof(T) == 8) v[s] = wave_sum_d(v[s]);
+    else v[s] = group_sum<64>(v[s]);
+  }
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
     for (int s = 0; s < S; ++s) red[flip][threadIdx.x >> 6][s] = v[s];
   }
   __syncthreads();
+  // (16 lanes read a value each and add them up by lane swaps: one read of LDS a wave and sum, not one for every other wave)
+  const int wave = threadIdx.x & 15;
 #pragma unroll
-  for (int s = 0; s < S; ++s) v[s] = 0.f;
-  for (int i = 0; i < waves; ++i) {
+  for (int s = 0; s < S; ++s) v[s] = wave < waves ? red[flip][wave][s] : (T)0;
 #pragma unroll
-    for (int s = 0; s < S; ++s) v[s] += red[flip][i][s];
+  for (int s = 0; s < S; ++s) {
+    if constexpr (sizeof(T) == 8) v[s] = row16_sum_d(v[s]);
+    else v[s] = group_sum<16>(v[s]);
   }
   flip ^= 1;
+}
+// a value of the row: the same in all lanes, and held once a wave, where the row is the workgroup's
+template <bool IN>
+__device__ __forceinline__ float row_value(float v) {
+  if constexpr (IN) return v;
+  else return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+// s / n by the reciprocal of n (inv, rounded) and the remainder of that quotient, which is exact: a quotient that is a float comes out exactly
+__device__ __forceinline__ float over(float s, float n, float inv) {
+  const float t = s * inv;
+  return fmaf(fmaf(-t, n, s), inv, t);
 }
 
 // TPR = 0: a workgroup a row (TPR = 1 024: one of that many threads, whose lanes have half the registers)
@@ -192,7 +216,7 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const Nor
   constexpr int V = Vec<TYPE>::N;
   constexpr bool IN = TPR > 0 && TPR <= 64;  // the row sits inside a wave
   constexpr int G = IN ? TPR : 64;
-  __shared__ float red[2][16][1];
+  __shared__ float red[2][16][2];
   const int lanes = IN ? G : blockDim.x, lane = IN ? threadIdx.x & (G - 1) : threadIdx.x;
   const int nv = A.cols / V, rest = nv * V + lane;  // full vectors of a row; this lane's element behind them
   const bool has_rest = rest < A.cols;
@@ -217,24 +241,31 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const Nor
 #pragma unroll
     for (int e = 0; e < NE * V; ++e) s[0] += x[e];
     if constexpr (IN) s[0] = group_sum<G>(s[0]);
-    else wg_sums<1>(s, red, flip);
-    const float mean = s[0] / (float)A.cols;  // (a division: the mean of a constant row is that constant)
-    float q2[1] = {0.f};
+    else wg_sums(s, red, flip);
+    const float mean = row_value<IN>(over(s[0], (float)A.cols, A.inv));
+    float q[2] = {0.f, 0.f};  // sums of the deviations from that, and of their squares
 #pragma unroll
-    for (int i = 0; i < NE; ++i)
+    for (int i = 0; i < NE; ++i) {
+      const float from = lane + i * lanes < nv ? mean : 0.f;  // (past the end x is 0)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = lane + i * lanes < nv ? x[i * V + j] - mean : 0.f;
+        const float d = x[i * V + j] - from;
         x[i * V + j] = d;
-        q2[0] = fmaf(d, d, q2[0]);
+        q[0] += d;
+        q[1] = fmaf(d, d, q[1]);
       }
+    }
     x[NE * V] = has_rest ? x[NE * V] - mean : 0.f;
-    q2[0] = fmaf(x[NE * V], x[NE * V], q2[0]);
-    if constexpr (IN) q2[0] = group_sum<G>(q2[0]);
-    else wg_sums<1>(q2, red, flip);
-    const float rstd = 1.f / sqrtf(q2[0] * A.inv + A.eps);
+    q[0] += x[NE * V];
+    q[1] = fmaf(x[NE * V], x[NE * V], q[1]);
+    if constexpr (IN) {
+      q[0] = group_sum<G>(q[0]);
+      q[1] = group_sum<G>(q[1]);
+    } else wg_sums(q, red, flip);
+    const float low = row_value<IN>(over(q[0], (float)A.cols, A.inv)), squares = fmaf(-low, q[0], q[1]);
+    const float rstd = row_value<IN>(1.f / sqrtf((squares < 0.f ? 0.f : squares) * A.inv + A.eps));  // (a NaN stays one)
     if (!on) continue;
-    if (lane == 0 && A.mean) { A.mean[row] = mean; A.rstd[row] = rstd; }
+    if (lane == 0 && A.mean) { A.mean[2 * row] = mean; A.mean[2 * row + 1] = low; A.rstd[row] = rstd; }
     const int64_t yo = row * A.cols;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
@@ -243,14 +274,14 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_kernel(const Nor
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float z = fmaf(x[i * V + j] * rstd, w[i * V + j], b[i * V + j]);
+          const float z = fmaf((x[i * V + j] - low) * rstd, w[i * V + j], b[i * V + j]);
           o[j] = z > 0.f ? z : z * A.slope;
         }
         vec_store<TYPE, ONCE>(A.y, yo + q * V, o);
       }
     }
     if (has_rest) {
-      const float z = fmaf(x[NE * V] * rstd, w[NE * V], b[NE * V]);
+      const float z = fmaf((x[NE * V] - low) * rstd, w[NE * V], b[NE * V]);
       el_store<TYPE>(A.y, yo + rest, z > 0.f ? z : z * A.slope);
     }
   }
@@ -274,11 +305,12 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   // (1 024 threads with 16 elements each have no registers for a row ahead: 6 000 x 8 199 fp32, both passes, 510 us with, 235 without)
   constexpr bool AHEAD = TPR != 1024 || NE * V < 16;
   Raw<NE> nx, ng;
-  float nmean = 0.f, nrstd = 0.f;
+  float nmean = 0.f, nlow = 0.f, nrstd = 0.f;
   if constexpr (AHEAD) {
     nx = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
     ng = raw_load<TYPE, NE, ONCE>(A.dy, row * A.lddy, lane, lanes, row < A.rows ? nv : 0, rest, row < A.rows && has_rest);
-    nmean = row < A.rows ? A.mean[row] : 0.f;
+    nmean = row < A.rows ? A.mean[2 * row] : 0.f;
+    nlow = row < A.rows ? A.mean[2 * row + 1] : 0.f;
     nrstd = row < A.rows ? A.rstd[row] : 0.f;
   }
   w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
@@ -291,25 +323,27 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
     if constexpr (!AHEAD) {
       nx = raw_load<TYPE, NE, ONCE>(A.x, row * A.ldx, lane, lanes, on ? nv : 0, rest, on && has_rest);
       ng = raw_load<TYPE, NE, ONCE>(A.dy, row * A.lddy, lane, lanes, on ? nv : 0, rest, on && has_rest);
-      nmean = on ? A.mean[row] : 0.f;
+      nmean = on ? A.mean[2 * row] : 0.f;
+      nlow = on ? A.mean[2 * row + 1] : 0.f;
       nrstd = on ? A.rstd[row] : 0.f;
     }
     float x[E], g[E];
     raw_values<TYPE, NE>(nx, x);
     raw_values<TYPE, NE>(ng, g);
-    const float mean = nmean, rstd = nrstd;
+    const float mean = row_value<IN>(nmean), low = row_value<IN>(nlow), rstd = row_value<IN>(nrstd);
     if constexpr (AHEAD) {
       const bool more = row + step < A.rows;
       nx = raw_load<TYPE, NE, ONCE>(A.x, (row + step) * A.ldx, lane, lanes, more ? nv : 0, rest, more && has_rest);
       ng = raw_load<TYPE, NE, ONCE>(A.dy, (row + step) * A.lddy, lane, lanes, more ? nv : 0, rest, more && has_rest);
-      nmean = more ? A.mean[row + step] : 0.f;
+      nmean = more ? A.mean[2 * (row + step)] : 0.f;
+      nlow = more ? A.mean[2 * (row + step) + 1] : 0.f;
       nrstd = more ? A.rstd[row + step] : 0.f;
     }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const bool there = e == E - 1 ? on && has_rest : on && lane + (e / V) * lanes < nv;
-      const float xh = there ? (x[e] - mean) * rstd : 0.f;  // (a lane past the end adds nothing, also where the mean is not finite)
+      const float xh = there ? (x[e] - mean - low) * rstd : 0.f;  // (a lane past the end adds nothing, also where the mean is not finite)
       if constexpr (ACT) g[e] = fmaf(xh, w[e], b[e]) > 0.f ? g[e] : g[e] * A.slope;
       const float gw = g[e] * w[e];
       s[0] += gw;
@@ -322,9 +356,9 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
     if constexpr (IN) {
       s[0] = group_sum<G>(s[0]);
       s[1] = group_sum<G>(s[1]);
-    } else wg_sums<2>(s, red, flip);
+    } else wg_sums(s, red, flip);
     if (!on || !A.dx) continue;
-    const float m0 = s[0] * A.inv, m1 = s[1] * A.inv;
+    const float m0 = row_value<IN>(s[0] * A.inv), m1 = row_value<IN>(s[1] * A.inv);
     const int64_t yo = row * A.cols;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
@@ -381,26 +415,28 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   }
 }
 
-// Rows too wide for the registers of 1 024 threads: the row is read again (from cache) for every step.
+// Rows too wide for the registers of 1 024 threads: the row is read again (from cache) for every step.  A thread adds up cols / 1 024
+// elements one after the other: forward in 64 bits.
 template <int TYPE>
 __global__ __launch_bounds__(1024) void layer_norm_wide_kernel(const NormArgs A) {
-  __shared__ float red[2][16][1];
+  __shared__ double red[2][16][1];
   int flip = 0;
   for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
     const int64_t xo = row * A.ldx;
-    float s[1] = {0.f}, q2[1] = {0.f};
-    for (int c = threadIdx.x; c < A.cols; c += 1024) s[0] += el_load<TYPE>(A.x, xo + c);
-    wg_sums<1>(s, red, flip);
-    const float mean = s[0] / (float)A.cols;  // (a division: the mean of a constant row is that constant)
+    double s[1] = {0.0}, q[1] = {0.0};
+    for (int c = threadIdx.x; c < A.cols; c += 1024) s[0] += (double)el_load<TYPE>(A.x, xo + c);
+    wg_sums(s, red, flip);
+    const double m = s[0] / (double)A.cols;
+    const float mean = (float)m, low = (float)(m - (double)mean);
     for (int c = threadIdx.x; c < A.cols; c += 1024) {
-      const float d = el_load<TYPE>(A.x, xo + c) - mean;
-      q2[0] = fmaf(d, d, q2[0]);
+      const double d = (double)(el_load<TYPE>(A.x, xo + c) - mean - low);
+      q[0] = fma(d, d, q[0]);
     }
-    wg_sums<1>(q2, red, flip);
-    const float rstd = 1.f / sqrtf(q2[0] * A.inv + A.eps);
-    if (threadIdx.x == 0 && A.mean) { A.mean[row] = mean; A.rstd[row] = rstd; }
+    wg_sums(q, red, flip);
+    const float rstd = (float)(1.0 / sqrt(q[0] / (double)A.cols + (double)A.eps));
+    if (threadIdx.x == 0 && A.mean) { A.mean[2 * row] = mean; A.mean[2 * row + 1] = low; A.rstd[row] = rstd; }
     for (int c = threadIdx.x; c < A.cols; c += 1024) {
-      const float z = fmaf((el_load<TYPE>(A.x, xo + c) - mean) * rstd, w_load(A.w, c, A.wtype, 1.f), w_load(A.b, c, A.wtype, 0.f));
+      const float z = fmaf((el_load<TYPE>(A.x, xo + c) - mean - low) * rstd, w_load(A.w, c, A.wtype, 1.f), w_load(A.b, c, A.wtype, 0.f));
       el_store<TYPE>(A.y, row * A.cols + c, z > 0.f ? z : z * A.slope);
     }
   }
@@ -414,10 +450,10 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const NormArg
   bool first = true;
   for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
     const int64_t xo = row * A.ldx, go = row * A.lddy;
-    const float mean = A.mean[row], rstd = A.rstd[row];
+    const float mean = A.mean[2 * row], low = A.mean[2 * row + 1], rstd = A.rstd[row];
     float s[2] = {0.f, 0.f};
     for (int c = threadIdx.x; c < A.cols; c += 1024) {
-      const float xh = (el_load<TYPE>(A.x, xo + c) - mean) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
+      const float xh = (el_load<TYPE>(A.x, xo + c) - mean - low) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
       float g = el_load<TYPE>(A.dy, go + c);
       if (A.slope != 1.f) g = fmaf(xh, w, w_load(A.b, c, A.wtype, 0.f)) > 0.f ? g : g * A.slope;
       s[0] += g * w;
@@ -428,11 +464,11 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const NormArg
       }
     }
     first = false;
-    wg_sums<2>(s, red, flip);
+    wg_sums(s, red, flip);
     if (!A.dx) continue;
     const float m0 = s[0] * A.inv, m1 = s[1] * A.inv;
     for (int c = threadIdx.x; c < A.cols; c += 1024) {
-      const float xh = (el_load<TYPE>(A.x, xo + c) - mean) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
+      const float xh = (el_load<TYPE>(A.x, xo + c) - mean - low) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
       float g = el_load<TYPE>(A.dy, go + c);
       if (A.slope != 1.f) g = fmaf(xh, w, w_load(A.b, c, A.wtype, 0.f)) > 0.f ? g : g * A.slope;
       el_store<TYPE>(A.dx, row * A.cols + c, rstd * (g * w - m0 - xh * m1));

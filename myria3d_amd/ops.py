@@ -1649,11 +1649,11 @@ def _layer_norm_fwd(rows: Tensor, shape, w: Optional[Tensor], b: Optional[Tensor
     n, cols = rows.shape
     dev = rows.device
     y = torch.empty(shape, dtype=rows.dtype, device=dev)
-    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if keep else None  # the rows' means, then 1 / deviation
+    stats = torch.empty((3, n), dtype=torch.float32, device=dev) if keep else None  # the rows' means (two floats each), then 1 / deviation
     at = stats.data_ptr() if keep else None
     with on_device(dev):
         call("m3d_layer_norm_fwd", rows.data_ptr(), rows.stride(0), _p(w), _p(b), n, cols, TYPES[rows.dtype], wtype, eps, slope,
-             y.data_ptr(), at, at and at + 4 * n, _st())
+             y.data_ptr(), at, at and at + 8 * n, _st())
     return y, stats
 
 
@@ -1687,7 +1687,7 @@ class LayerNormFn(torch.autograd.Function):
             ws = torch.empty(lib().m3d_layer_norm_bwd_workspace_bytes(n, cols, xtype), dtype=torch.uint8, device=dev)
         at = stats.data_ptr()
         with on_device(dev):
-            call("m3d_layer_norm_bwd", dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), _p(w), _p(b), at, at + 4 * n, n, cols,
+            call("m3d_layer_norm_bwd", dy.data_ptr(), dy.stride(0), rows.data_ptr(), rows.stride(0), _p(w), _p(b), at, at + 8 * n, n, cols,
                  xtype, wtype, slope, _p(dx), _p(dw), _p(db), _p(ws), _st())
         return dx, dw, db, None, None, None
 
