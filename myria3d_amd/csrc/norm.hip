@@ -16,9 +16,10 @@
 // A row belongs to TPR lanes, each with NE vectors of 16 bytes (4 fp32 or 8 half-precision elements) and, where the width is not
 // a multiple of a vector, one element of the rest.  Up to 64 lanes the row sits inside a wave (narrow rows: several rows a wave,
 // sums by lane swaps, no LDS); above, a workgroup of 128 to 1 024 threads takes a row (sums over its waves through LDS).  The
-// columns of a lane are the same for every row it meets: w and b are read once per lane, and the backward pass keeps dw and db of
-// its columns in registers over all its rows.  At the end the waves of a workgroup are added up through LDS in a fixed order, the
-// workgroups leave one row of partial sums each, and a second kernel adds these in 64 bits: no atomics, the same bits every time.
+// columns of a lane are the same for every row it meets: w and b are read once per lane (where they fit), and the backward pass
+// keeps dw and db of its columns in registers over all its rows.  At the end the waves of a workgroup are added up through LDS in a
+// fixed order, the workgroups leave one row of partial sums each, and a second kernel adds these in 64 bits: no atomics, the same bits
+// every time.
 // Vectors are loaded with the alignment of their element, so rows of any stride take this path.
 //
 // Bound by memory (6.1 TB/s is what a large scaling reaches here): 1 638 400 x 64 fp32 forward 147 us, 5.7 TB/s, backward 203 + 5 us,
@@ -119,29 +120,30 @@ __device__ __forceinline__ float w_load(const void* base, int64_t e, int type, f
   if (!base) return none;
   return type == M3D_TYPE_F32 ? el_load<M3D_TYPE_F32>(base, e) : type == M3D_TYPE_BF16 ? el_load<M3D_TYPE_BF16>(base, e) : el_load<M3D_TYPE_F16>(base, e);
 }
-// the weights of a lane's columns (vectors of V elements, then the one of the rest)
-template <int V, int NE>
-__device__ __forceinline__ void w_loads(const void* base, int type, float none, int lane, int lanes, int nv, int rest, bool has_rest, float* w) {
+// the weights of a lane's columns: a vector of V elements (vector q of the row's nv; shift: 0), all NE of them and the one of the rest
+template <int V>
+__device__ __forceinline__ void w_vector(const void* base, int type, float none, int q, int nv, float* w, uint32_t shift = 0u) {
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int q = lane + i * lanes;
+  for (int j = 0; j < V; j += 4) {
+    float* o = w + j;
+    o[0] = o[1] = o[2] = o[3] = q < nv ? none : 0.f;
+    if (base && q < nv) {
+      if (type == M3D_TYPE_F32) {
+        const f4u t = *(const f4u*)((const float*)base + ((uint32_t)(q * V + j) + shift));
 #pragma unroll
-    for (int j = 0; j < V; j += 4) {
-      float* o = w + i * V + j;
-      o[0] = o[1] = o[2] = o[3] = q < nv ? none : 0.f;
-      if (base && q < nv) {
-        if (type == M3D_TYPE_F32) {
-          const f4u t = *(const f4u*)((const float*)base + q * V + j);
+        for (int k = 0; k < 4; ++k) o[k] = t[k];
+      } else {
+        const h4u t = *(const h4u*)((const unsigned short*)base + ((uint32_t)(q * V + j) + shift));
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = t[k];
-        } else {
-          const h4u t = *(const h4u*)((const unsigned short*)base + q * V + j);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = type == M3D_TYPE_BF16 ? bf16_to_f32(t[k]) : (float)__builtin_bit_cast(_Float16, (unsigned short)t[k]);
-        }
+        for (int k = 0; k < 4; ++k) o[k] = type == M3D_TYPE_BF16 ? bf16_to_f32(t[k]) : (float)__builtin_bit_cast(_Float16, (unsigned short)t[k]);
       }
     }
   }
+}
+template <int V, int NE>
+__device__ __forceinline__ void w_loads(const void* base, int type, float none, int lane, int lanes, int nv, int rest, bool has_rest, float* w) {
+#pragma unroll
+  for (int i = 0; i < NE; ++i) w_vector<V>(base, type, none, lane + i * lanes, nv, w + i * V);
   w[NE * V] = has_rest ? w_load(base, rest, type, none) : 0.f;
 }
 
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   constexpr int G = IN ? TPR : 64;
   __shared__ float red[2][16][2];
   extern __shared__ __attribute__((aligned(16))) float sums[];  // IN: the waves' dw and db
-  const int lanes = IN ? G : blockDim.x, lane = IN ? threadIdx.x & (G - 1) : threadIdx.x;
+  const int lanes = IN ? G : TPR == 1024 ? 1024 : blockDim.x, lane = IN ? threadIdx.x & (G - 1) : threadIdx.x;
   const int nv = A.cols / V, rest = nv * V + lane;
   const bool has_rest = rest < A.cols;
   float w[E], b[E], dw[E], db[E];  // (b only to find the sign of z again)
@@ -302,7 +304,9 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
   const int64_t step = (int64_t)gridDim.x * per;
   int64_t row = (int64_t)blockIdx.x * per + (IN ? threadIdx.x / G : 0);
   const int64_t turns = (A.rows - (int64_t)blockIdx.x * per + step - 1) / step;
-  // (1 024 threads with 16 elements each have no registers for a row ahead: 6 000 x 8 199 fp32, both passes, 510 us with, 235 without)
+  // 1 024 threads with 16 elements each have 128 registers a lane: none for a row ahead (6 000 x 8 199 fp32, both passes: 510 us with one),
+  // nor for w and b, which are read again with every row (with the activation 265 us where they were kept and went to scratch
+  // memory, 237 now; without it 233 and 228).
   constexpr bool AHEAD = TPR != 1024 || NE * V < 16;
   Raw<NE> nx, ng;
   float nmean = 0.f, nlow = 0.f, nrstd = 0.f;
@@ -313,8 +317,10 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
     nlow = row < A.rows ? A.mean[2 * row + 1] : 0.f;
     nrstd = row < A.rows ? A.rstd[row] : 0.f;
   }
-  w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
-  if constexpr (ACT) w_loads<V, NE>(A.b, A.wtype, 0.f, lane, lanes, nv, rest, has_rest, b);
+  if constexpr (AHEAD) {
+    w_loads<V, NE>(A.w, A.wtype, 1.f, lane, lanes, nv, rest, has_rest, w);
+    if constexpr (ACT) w_loads<V, NE>(A.b, A.wtype, 0.f, lane, lanes, nv, rest, has_rest, b);
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
   int flip = 0;
@@ -340,8 +346,21 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
       nrstd = more ? A.rstd[row + step] : 0.f;
     }
     float s[2] = {0.f, 0.f};
+    uint32_t zero = 0u;
+    if constexpr (!AHEAD) asm volatile("" : "+s"(zero));  // (or the compiler would keep the addresses of w and b, 40 registers, over the rows)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+      if constexpr (!AHEAD) {
+        if (e == E - 1) {
+          const uint32_t at = (uint32_t)(nv * V + lane) + zero;
+          w[e] = has_rest ? w_load(A.w, at, A.wtype, 1.f) : 0.f;
+          if constexpr (ACT) b[e] = has_rest ? w_load(A.b, at, A.wtype, 0.f) : 0.f;
+        } else if (e % 4 == 0) {
+          const int q = (lane + (e / V) * lanes) * (V / 4) + e % V / 4;
+          w_vector<4>(A.w, A.wtype, 1.f, q, nv * (V / 4), w + e, zero);
+          if constexpr (ACT) w_vector<4>(A.b, A.wtype, 0.f, q, nv * (V / 4), b + e, zero);
+        }
+      }
       const bool there = e == E - 1 ? on && has_rest : on && lane + (e / V) * lanes < nv;
       const float xh = there ? (x[e] - mean - low) * rstd : 0.f;  // (a lane past the end adds nothing, also where the mean is not finite)
       if constexpr (ACT) g[e] = fmaf(xh, w[e], b[e]) > 0.f ? g[e] : g[e] * A.slope;
