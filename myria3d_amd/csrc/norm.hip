@@ -435,7 +435,7 @@ __global__ __launch_bounds__(NORM_THREADS(TPR)) void layer_norm_bwd_kernel(const
 }
 
 // Rows too wide for the registers of 1 024 threads: the row is read again (from cache) for every step.  A thread adds up cols / 1 024
-// elements one after the other: forward in 64 bits.
+// elements one after the other, so the row's sums are in 64 bits.
 template <int TYPE>
 __global__ __launch_bounds__(1024) void layer_norm_wide_kernel(const NormArgs A) {
   __shared__ double red[2][16][1];
@@ -463,20 +463,20 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_kernel(const NormArgs A)
 // (dw and db: a workgroup owns a run of rows AND walks all columns, adding to its own row of partial sums)
 template <int TYPE>
 __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const NormArgs A) {
-  __shared__ float red[2][16][2];
+  __shared__ double red[2][16][2];
   int flip = 0;
   float* out = A.parts ? A.parts + (int64_t)blockIdx.x * 2 * A.cols : nullptr;
   bool first = true;
   for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
     const int64_t xo = row * A.ldx, go = row * A.lddy;
     const float mean = A.mean[2 * row], low = A.mean[2 * row + 1], rstd = A.rstd[row];
-    float s[2] = {0.f, 0.f};
+    double s[2] = {0.0, 0.0};
     for (int c = threadIdx.x; c < A.cols; c += 1024) {
       const float xh = (el_load<TYPE>(A.x, xo + c) - mean - low) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
       float g = el_load<TYPE>(A.dy, go + c);
       if (A.slope != 1.f) g = fmaf(xh, w, w_load(A.b, c, A.wtype, 0.f)) > 0.f ? g : g * A.slope;
-      s[0] += g * w;
-      s[1] = fmaf(g * w, xh, s[1]);
+      s[0] += (double)(g * w);
+      s[1] = fma((double)(g * w), (double)xh, s[1]);
       if (out) {
         out[c] = first ? g * xh : fmaf(g, xh, out[c]);
         out[A.cols + c] = first ? g : out[A.cols + c] + g;
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const NormArg
     first = false;
     wg_sums(s, red, flip);
     if (!A.dx) continue;
-    const float m0 = s[0] * A.inv, m1 = s[1] * A.inv;
+    const float m0 = (float)(s[0] / (double)A.cols), m1 = (float)(s[1] / (double)A.cols);
     for (int c = threadIdx.x; c < A.cols; c += 1024) {
       const float xh = (el_load<TYPE>(A.x, xo + c) - mean - low) * rstd, w = w_load(A.w, c, A.wtype, 1.f);
       float g = el_load<TYPE>(A.dy, go + c);

@@ -102,3 +102,21 @@ def test_both_passes_see_the_same_side_of_the_activation():
         y = myria3d_amd.layer_norm(x, w, b, negative_slope=0.0)
         (db,) = torch.autograd.grad(y, b, torch.ones_like(y))
         assert torch.equal(db, (y > 0).sum(0).float()), cols
+
+
+@pytest.mark.parametrize("cols", [1 << 20, 3000001])
+def test_sums_over_many_columns(cols):
+    """Equal terms add up with roundings of one sign: one thread's thousands of columns in 32 bits would miss the bound three times over."""
+    import myria3d_amd
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = (torch.randn(3, cols, generator=g, device="cuda") + 100.0).requires_grad_()
+    w, b = torch.ones(cols, device="cuda", requires_grad=True), torch.zeros(cols, device="cuda", requires_grad=True)
+    dy = torch.full((3, cols), 0.1, device="cuda")
+    dy[1] = 0.1 * (x[1].detach() - 100.0) + 0.1
+    dy[2] = torch.randn(cols, generator=g, device="cuda")
+    y = myria3d_amd.layer_norm(x, w, b)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, (x, w, b), dy)), y=y.detach())
+    for name, (value, bound) in bounds(x, w, b, 1e-5, dy).items():
+        worst = ((got[name].double() - value).abs() / bound).max().item()
+        assert worst <= 1.0, (name, worst)
