@@ -12,6 +12,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ._lib import call, lib
 
@@ -1646,7 +1647,7 @@ def _rows_of(t: Tensor) -> Tensor:
 
 
 def _layer_norm_fwd(rows: Tensor, shape, w: Optional[Tensor], b: Optional[Tensor], wtype: int, eps: float, slope: float, keep: bool):
-    n, cols = rows.shape
+    n, cols = map(int, rows.shape)  # (tensors in a trace)
     dev = rows.device
     y = torch.empty(shape, dtype=rows.dtype, device=dev)
     stats = torch.empty((3, n), dtype=torch.float32, device=dev) if keep else None  # the rows' means (two floats each), then 1 / deviation
@@ -1697,7 +1698,8 @@ class LayerNormFn(torch.autograd.Function):
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
                negative_slope: Optional[float] = None) -> Tensor:
     """``torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)``, differentiable (once) in ``x``, ``weight`` and
-    ``bias``; with ``negative_slope`` the LeakyReLU that follows it, in the same pass over the data.
+    ``bias`` by backward passes (forward-mode differentiation and ``torch.func`` raise); with ``negative_slope`` the LeakyReLU that
+    follows it, in the same pass over the data.
 
     ``x``: fp32, bf16 or fp16, any shape whose last dimension is not empty; rows may have a stride of their own (a slice of a wider
     matrix is read in place, an order with other than the last dimension innermost is copied).  ``weight`` / ``bias``: contiguous,
@@ -1725,8 +1727,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     if not x.is_cuda:
         raise RuntimeError("layer_norm runs on an MI355X only (no CPU fallback by design)")
     wtype = TYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype]
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    # (a trace records the function, and forward-mode differentiation finds that it has no tangent: a bare launch would show neither)
+    if torch.jit.is_tracing() or forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return LayerNormFn.apply(x, weight, bias, wtype, float(eps), slope)
     return _layer_norm_fwd(_rows_of(x), x.shape, weight, bias, wtype, float(eps), slope, False)[0]
 
