@@ -464,8 +464,9 @@ class AdamW(torch.optim.Optimizer):
                     a.lr_dev, a.lr = None, lr
                 a.beta1, a.beta2, a.eps, a.weight_decay = b1, b2, group["eps"], group["weight_decay"]
                 call("m3d_adamw_step", ctypes.addressof(a), st)
-                # (the parameters changed behind torch's back: caches that go by their version counters notice)
-                torch.autograd.graph.increment_version(g.params)
+                # (these parameters changed behind torch's back: graphs and caches that go by their version counters notice.  Whether a
+                # clipped step was taken only the device knows: its parameters count as changed)
+                torch.autograd.graph.increment_version(g.params if all(ptrs) else [p for p, x in zip(g.params, ptrs) if x])
         return loss
 
     # ------------------------------------------------------------------------------------------
