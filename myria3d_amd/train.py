@@ -11,6 +11,7 @@
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
 from array import array
@@ -528,11 +529,13 @@ class AdamW(torch.optim.Optimizer):
             g.state.zero_()
             g.state[0] = top
             g.missed.copy_(torch.tensor([int(top - s) for s in steps], dtype=torch.int32))
-            for k, v in group.items():
+            for k, v in group.items():  # (all of it, as torch does: a scheduler made after this looks for initial_lr)
                 if k == "lr" and isinstance(mine["lr"], Tensor):
                     mine["lr"].fill_(float(v))  # (the place that a captured step reads)
-                elif k != "params" and k in mine:
-                    mine[k] = float(v) if isinstance(v, Tensor) else v
+                elif k == "betas":
+                    mine[k] = tuple(float(b) for b in v)
+                elif k != "params" and not (k == "param_names" and k in mine):
+                    mine[k] = float(v) if isinstance(v, Tensor) else copy.deepcopy(v)
 
     def __getstate__(self):
         raise TypeError("AdamW cannot be copied or pickled: make another one and load state_dict()")

@@ -42,3 +42,26 @@ def test_a_parameter_without_a_gradient_is_not_changed(bits, max_grad_norm):
     a.grad = None
     opt.step()
     assert [p._version for p in (a, b, c)] == nothing
+
+
+@pytest.mark.parametrize("tensor_lr", [False, True])
+def test_a_schedule_goes_on_after_loading(tensor_lr):
+    """What a scheduler leaves in a group travels with the state, as in torch: here and from torch's own optimizer."""
+    import myria3d_amd
+    from torch.optim.lr_scheduler import StepLR
+
+    for make in (lambda p: myria3d_amd.AdamW([p], lr=0.5), lambda p: torch.optim.AdamW([p], lr=0.5, betas=(0.8, 0.99))):
+        p, q = _param(30, seed=4), _param(30, seed=4)
+        first = make(p)
+        sched = StepLR(first, 1, 0.5)
+        for _ in range(2):
+            first.step(), sched.step()
+        second = myria3d_amd.AdamW([q], lr=torch.tensor(7.0, device="cuda") if tensor_lr else 7.0)
+        second.load_state_dict(first.state_dict())
+        assert second.param_groups[0]["betas"] == first.param_groups[0]["betas"]
+        again = StepLR(second, 1, 0.5, last_epoch=2)  # (takes its first step by itself)
+        sched.step()
+        assert again.base_lrs == [0.5] and float(second.param_groups[0]["lr"]) == float(first.param_groups[0]["lr"]) == 0.0625
+        saved = second.state_dict()["param_groups"][0]
+        assert saved["initial_lr"] == 0.5 and saved["params"] == [0]
+    torch.optim.AdamW([q]).load_state_dict(second.state_dict())
