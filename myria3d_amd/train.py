@@ -342,7 +342,7 @@ class AdamW(torch.optim.Optimizer):
     ``lr`` may be a 0-dim fp32 tensor on the device (a schedule under graph replay).  Nothing is read back and step counts live on the
     device: ``step()`` may be captured into a hipGraph (after one eager step) and replayed; the gradients must then be written in
     place.  ``state_dict()`` has torch's layout (``step``, ``exp_avg``, ``exp_avg_sq`` per parameter), and with 32 bits states travel
-    to and from ``torch.optim.AdamW`` / ``Adam``; with 8 bits the codes and scales are stored, and 32-bit states are taken in too."""
+    to and from ``torch.optim.AdamW`` and, without a weight decay of its own kind, ``Adam``; with 8 bits the codes and scales are stored, and 32-bit states are taken in too."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, max_grad_norm: Optional[float] = None):
@@ -354,7 +354,8 @@ class AdamW(torch.optim.Optimizer):
         self._groups: List[_Group] = []
         self._device = None
         self.grad_norm: Optional[Tensor] = None
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        # (the last one is torch's mark of AdamW's decay, by which torch.optim.Adam goes on with that where it loads this state)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled_weight_decay=True))
         if self.max_grad_norm is not None:
             self.grad_norm = torch.zeros((), dtype=torch.float32, device=self._device)
             self._parts = torch.empty(GRAD_NORM_PARTS, dtype=torch.float64, device=self._device)
@@ -498,6 +499,8 @@ class AdamW(torch.optim.Optimizer):
         for g, group in zip(self._groups, groups):
             if group.get("amsgrad", False) or group.get("maximize", False):
                 raise ValueError("AdamW implements amsgrad=False, maximize=False only")
+            if not group.get("decoupled_weight_decay", True) and float(group.get("weight_decay", 0.0)) != 0.0:
+                raise ValueError("the state of an optimizer whose weight decay goes through the gradient (Adam's) cannot go on with AdamW's")
             entries = [state.get(key, state.get(str(key))) for key in group["params"]]
             coded = {("exp_avg_scale" in e) for e in entries if e}
             for p, e in zip(g.params, entries):
@@ -534,7 +537,7 @@ class AdamW(torch.optim.Optimizer):
                     mine["lr"].fill_(float(v))  # (the place that a captured step reads)
                 elif k == "betas":
                     mine[k] = tuple(float(b) for b in v)
-                elif k != "params" and not (k == "param_names" and k in mine):
+                elif k not in ("params", "decoupled_weight_decay") and not (k == "param_names" and k in mine):
                     mine[k] = float(v) if isinstance(v, Tensor) else copy.deepcopy(v)
 
     def __getstate__(self):

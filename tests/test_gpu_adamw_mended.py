@@ -65,3 +65,30 @@ def test_a_schedule_goes_on_after_loading(tensor_lr):
         saved = second.state_dict()["param_groups"][0]
         assert saved["initial_lr"] == 0.5 and saved["params"] == [0]
     torch.optim.AdamW([q]).load_state_dict(second.state_dict())
+
+
+def test_weight_decay_stays_of_its_kind():
+    """Adam adds its decay to the gradient, AdamW takes it from the parameter: neither goes on as the other without a word."""
+    import myria3d_amd
+
+    p, q = _param(30, seed=5), _param(30, seed=5)
+    theirs = torch.optim.Adam([p], lr=0.1, weight_decay=0.5)
+    theirs.step()
+    opt = myria3d_amd.AdamW([q], lr=7.0)
+    before = opt.state_dict()
+    with pytest.raises(ValueError, match="decay"):
+        opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["lr"] == 7.0 and torch.equal(opt.state_dict()["state"][0]["exp_avg"], before["state"][0]["exp_avg"])
+    plain = torch.optim.Adam([p], lr=0.1)  # without decay there is no difference
+    plain.step()
+    opt.load_state_dict(plain.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.1 and opt.param_groups[0]["weight_decay"] == 0.0
+    with torch.no_grad():
+        q.copy_(p)
+    opt.param_groups[0]["weight_decay"] = 0.5
+    saved = opt.state_dict()
+    other = torch.optim.Adam([p], weight_decay=0.5, foreach=False)
+    other.load_state_dict(saved)
+    other.step(), opt.step()
+    # both decoupled now, each within 16 roundings of p and of an update of at most 10 lr; Adam's own would differ by some 0.1
+    assert bool(((p - q).abs() <= 2 * 16 * U * (q.abs() + 1.0)).all())
