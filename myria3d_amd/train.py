@@ -277,7 +277,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
 class _Group:
     """What one parameter group of ``AdamW`` keeps: sizes and types of its tensors, its moments (flat, in blocks of 256), counters."""
 
-    def __init__(self, params: List[Tensor], bits: int):
+    def __init__(self, params: List[Tensor], bits: int, dev: torch.device):
         self.params, self.bits = params, bits
         self.numel, self.types = _sizes(params), _types(params, "AdamW: parameters")
         self.strides = [p.stride() for p in params]
@@ -287,7 +287,6 @@ class _Group:
             self.starts.append(blocks * BLOCK)
             blocks += -(-p.numel() // BLOCK)
         self.blocks = blocks
-        dev = params[0].device
         self.avg, self.avg_sq = (torch.zeros(blocks * BLOCK, dtype=torch.float32 if bits == 32 else torch.uint8, device=dev) for _ in range(2))
         self.scale = self.scale_sq = None
         if bits == 8:
@@ -351,11 +350,14 @@ class AdamW(torch.optim.Optimizer):
         if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
             raise ValueError(f"AdamW: max_grad_norm must not be negative, got {max_grad_norm}")
         self.state_bits, self.max_grad_norm = state_bits, None if max_grad_norm is None else float(max_grad_norm)
-        self._groups: List[_Group] = []
+        self._groups: List[_Group] = []  # (None, until a device is known, for one without parameters)
         self._device = None
         self.grad_norm: Optional[Tensor] = None
         # (the last one is torch's mark of AdamW's decay, by which torch.optim.Adam goes on with that where it loads this state)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled_weight_decay=True))
+        if self._device is None:
+            raise ValueError("AdamW: no parameters")
+        self._groups = [g if g is not None else _Group([], state_bits, self._device) for g in self._groups]
         if self.max_grad_norm is not None:
             self.grad_norm = torch.zeros((), dtype=torch.float32, device=self._device)
             self._parts = torch.empty(GRAD_NORM_PARTS, dtype=torch.float64, device=self._device)
@@ -379,13 +381,11 @@ class AdamW(torch.optim.Optimizer):
         group = self.param_groups[-1]
         try:
             params = group["params"]
-            if not params:
-                raise ValueError("AdamW: a parameter group without parameters")
             self._check_group(group)
             if len({id(p) for p in params}) < len(params):
                 raise ValueError("AdamW: the same parameter twice in a group")
-            dev = self._device or params[0].device
-            if isinstance(group["lr"], Tensor) and group["lr"].device != dev:
+            dev = self._device or (params[0].device if params else None)
+            if params and isinstance(group["lr"], Tensor) and group["lr"].device != dev:
                 raise ValueError("AdamW: a tensor lr must be one fp32 element on the parameters' device")
             for p in params:
                 if p.dtype not in ops.TYPES:
@@ -398,7 +398,7 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
         self._device = dev
-        self._groups.append(_Group(list(params), self.state_bits))
+        self._groups.append(None if dev is None else _Group(list(params), self.state_bits, dev))
 
     # ------------------------------------------------------------------------------------------
     def _parameters(self, g: _Group) -> array:
@@ -455,6 +455,8 @@ class AdamW(torch.optim.Optimizer):
                     numel, types, grads = numel + g.numel, types + g.types, grads + ptrs
                 call("m3d_grad_norm", _at(grads), _at(numel), _at(types), len(grads), self._parts.data_ptr(), ctypes.addressof(nparts), st)
             for g, group, (params, ptrs) in zip(self._groups, self.param_groups, pointers):
+                if not g.params:
+                    continue
                 lr, (b1, b2) = group["lr"], group["betas"]
                 a = g.args
                 a.params, a.grads = _at(params), _at(ptrs)

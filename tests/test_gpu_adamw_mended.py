@@ -92,3 +92,29 @@ def test_weight_decay_stays_of_its_kind():
     other.step(), opt.step()
     # both decoupled now, each within 16 roundings of p and of an update of at most 10 lr; Adam's own would differ by some 0.1
     assert bool(((p - q).abs() <= 2 * 16 * U * (q.abs() + 1.0)).all())
+
+
+@pytest.mark.parametrize("bits, max_grad_norm", [(32, None), (8, 0.5)])
+def test_groups_without_parameters(bits, max_grad_norm):
+    """As torch takes them: in front of, between and behind the others, with a state that travels, and all alone not at all."""
+    import myria3d_amd
+
+    p, q = _param(300, seed=6), _param(300, seed=6)
+    alone = myria3d_amd.AdamW([q], lr=0.1, state_bits=bits, max_grad_norm=max_grad_norm)
+    opt = myria3d_amd.AdamW([{"params": [], "lr": 3.0}, {"params": [p], "lr": 0.1}], state_bits=bits, max_grad_norm=max_grad_norm)
+    opt.add_param_group({"params": []})
+    for _ in range(2):
+        opt.step(), alone.step()
+    assert torch.equal(p, q) and [len(g["params"]) for g in opt.param_groups] == [0, 1, 0]
+    if max_grad_norm is not None:
+        assert torch.equal(opt.grad_norm, alone.grad_norm)
+    saved = opt.state_dict()
+    assert [g["params"] for g in saved["param_groups"]] == [[], [0], []] and list(saved["state"]) == [0]
+    again = myria3d_amd.AdamW([{"params": []}, {"params": [p]}, {"params": []}], state_bits=bits, max_grad_norm=max_grad_norm)
+    again.load_state_dict(saved)
+    assert [g["lr"] for g in again.param_groups] == [3.0, 0.1, 1e-3]
+    again.step(), alone.step()
+    assert torch.equal(p, q)
+    assert [tuple(m.numel() for m in pair) for pair in again.moments()] == [(0, 0), (512, 512), (0, 0)]
+    with pytest.raises(ValueError):
+        myria3d_amd.AdamW([{"params": []}, {"params": []}], state_bits=bits)
