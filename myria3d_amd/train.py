@@ -492,28 +492,48 @@ class AdamW(torch.optim.Optimizer):
             groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": index})
         return {"state": state, "param_groups": groups}
 
+    @staticmethod
+    def _check_entry(p: Tensor, e: dict, coded: bool) -> None:
+        keys = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if coded else set())
+        if not keys <= set(e):
+            raise ValueError(f"optimizer state lacks {sorted(keys - set(e))}")
+        for key in ("exp_avg", "exp_avg_sq"):
+            m = e[key]
+            if tuple(m.shape) != tuple(p.shape):
+                raise ValueError(f"optimizer state has shape {tuple(m.shape)}, expected {tuple(p.shape)}")
+            if m.dtype != torch.uint8 if coded else not m.is_floating_point():
+                raise ValueError(f"optimizer state {key} has type {m.dtype}, expected {'uint8' if coded else 'a floating-point type'}")
+            if coded:
+                if not (m.is_contiguous() and p.is_contiguous()) and m.stride() != p.stride():
+                    raise ValueError("8-bit states belong to the memory order of the parameter that they were saved from")
+                s, blocks = e[key + "_scale"], -(-p.numel() // BLOCK)
+                if tuple(s.shape) != (blocks,) or not s.is_floating_point():
+                    raise ValueError(f"optimizer state has {s.dtype} scales of shape {tuple(s.shape)}, expected {(blocks,)}")
+
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         groups, state = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g.params) for g in self._groups]:
             raise ValueError("loaded state dict has other parameter groups")
-        todo = []
-        for g, group in zip(self._groups, groups):
+        todo = []  # (all of it is looked at before any of it is written)
+        for g, group, mine in zip(self._groups, groups, self.param_groups):
             if group.get("amsgrad", False) or group.get("maximize", False):
                 raise ValueError("AdamW implements amsgrad=False, maximize=False only")
             if not group.get("decoupled_weight_decay", True) and float(group.get("weight_decay", 0.0)) != 0.0:
                 raise ValueError("the state of an optimizer whose weight decay goes through the gradient (Adam's) cannot go on with AdamW's")
             entries = [state.get(key, state.get(str(key))) for key in group["params"]]
             coded = {("exp_avg_scale" in e) for e in entries if e}
-            for p, e in zip(g.params, entries):
-                if e and tuple(e["exp_avg"].shape) != tuple(p.shape):
-                    raise ValueError(f"optimizer state has shape {tuple(e['exp_avg'].shape)}, expected {tuple(p.shape)}")
-                if e and "exp_avg_scale" in e and not (e["exp_avg"].is_contiguous() and p.is_contiguous()) and e["exp_avg"].stride() != p.stride():
-                    raise ValueError("8-bit states belong to the memory order of the parameter that they were saved from")
             if len(coded) > 1 or (True in coded and g.bits != 8):
                 raise ValueError("8-bit states go into an optimizer with state_bits=8 only")
-            todo.append((g, group, entries, True in coded))
-        for (g, group, entries, coded), mine in zip(todo, self.param_groups):
+            for p, e in zip(g.params, entries):
+                if e:
+                    self._check_entry(p, e, True in coded)
+            # (everything in the group, as torch does: a scheduler made after this looks for initial_lr)
+            values = {k: tuple(map(float, v)) if k == "betas" else float(v) if isinstance(v, Tensor) else copy.deepcopy(v)
+                      for k, v in group.items() if k not in ("params", "decoupled_weight_decay") and not (k == "param_names" and k in mine)}
+            self._check_group({**mine, **values})
+            todo.append((g, mine, values, entries, True in coded))
+        for g, mine, values, entries, coded in todo:
             steps = [float(e["step"]) if e else 0.0 for e in entries]
             top = max(steps, default=0.0)
             if coded or g.bits == 32:
@@ -534,13 +554,11 @@ class AdamW(torch.optim.Optimizer):
             g.state.zero_()
             g.state[0] = top
             g.missed.copy_(torch.tensor([int(top - s) for s in steps], dtype=torch.int32))
-            for k, v in group.items():  # (all of it, as torch does: a scheduler made after this looks for initial_lr)
+            for k, v in values.items():
                 if k == "lr" and isinstance(mine["lr"], Tensor):
-                    mine["lr"].fill_(float(v))  # (the place that a captured step reads)
-                elif k == "betas":
-                    mine[k] = tuple(float(b) for b in v)
-                elif k not in ("params", "decoupled_weight_decay") and not (k == "param_names" and k in mine):
-                    mine[k] = float(v) if isinstance(v, Tensor) else copy.deepcopy(v)
+                    mine["lr"].fill_(v)  # (the place that a captured step reads)
+                else:
+                    mine[k] = v
 
     def __getstate__(self):
         raise TypeError("AdamW cannot be copied or pickled: make another one and load state_dict()")

@@ -118,3 +118,43 @@ def test_groups_without_parameters(bits, max_grad_norm):
     assert [tuple(m.numel() for m in pair) for pair in again.moments()] == [(0, 0), (512, 512), (0, 0)]
     with pytest.raises(ValueError):
         myria3d_amd.AdamW([{"params": []}, {"params": []}], state_bits=bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_that_does_not_fit_changes_nothing(bits):
+    import copy
+
+    import myria3d_amd
+
+    params = [_param(30, 40, seed=7), _param(700, seed=8)]
+    opt = myria3d_amd.AdamW([{"params": params[:1]}, {"params": params[1:]}], lr=0.1, state_bits=bits)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+
+    def broken(change):
+        d = copy.deepcopy(saved)
+        d["param_groups"][0]["lr"] = 0.7
+        d["state"][0]["exp_avg"].fill_(3)
+        change(d)
+        return d
+
+    changes = [lambda d: d["state"][1].pop("exp_avg_sq"), lambda d: d["state"][1].pop("step"),
+               lambda d: d["state"][1].update(exp_avg_sq=d["state"][1]["exp_avg_sq"][:1]),  # (one that would spread over all of it)
+               lambda d: d["state"][1].update(exp_avg=d["state"][1]["exp_avg"].int()),
+               lambda d: d["param_groups"][1].update(betas=(0.9, 1.5)), lambda d: d["param_groups"][1].update(lr=-1.0)]
+    if bits == 8:
+        changes += [lambda d: d["state"][1].update(exp_avg_scale=d["state"][1]["exp_avg_scale"][:1]),
+                    lambda d: d["state"][1].pop("exp_avg_sq_scale"), lambda d: d["state"][1].pop("exp_avg_scale"),
+                    lambda d: d["state"][1].update(exp_avg_sq=d["state"][1]["exp_avg_sq"].float())]
+    for k, change in enumerate(changes):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(broken(change))
+        now = opt.state_dict()
+        assert now["param_groups"] == saved["param_groups"], k
+        for i in (0, 1):
+            assert all(torch.equal(torch.as_tensor(v), torch.as_tensor(saved["state"][i][name])) for name, v in now["state"][i].items()), (k, i)
+    lr = torch.tensor(0.25)  # what torch's capturable optimizers leave in a group
+    saved["param_groups"][0].update(lr=lr, betas=[0.5, 0.75])
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["betas"] == (0.5, 0.75)
+    opt.step()
