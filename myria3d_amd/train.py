@@ -226,6 +226,13 @@ def _check_strided(tensors: List[Tensor]) -> None:
         raise RuntimeError("sparse gradients are not supported")
 
 
+def _check_apart(params: List[Tensor]) -> None:
+    """Whether no two of these (dense) parameters share memory: both would be updated at once."""
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+    if any(stop > start for (_, stop), (start, _) in zip(spans, spans[1:])):
+        raise ValueError("AdamW: two parameters of a group share memory")
+
+
 def _at(a: array) -> int:
     return a.buffer_info()[0]
 
@@ -394,6 +401,7 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"AdamW: a parameter's elements must fill one run of memory, got strides {p.stride()} for {tuple(p.shape)}")
                 if p.device != dev or p.device.type != "cuda":
                     raise RuntimeError(f"AdamW: all parameters must be on one MI355X (no CPU fallback by design), got {p.device} and {dev}")
+            _check_apart(params)
         except Exception:
             self.param_groups.pop()
             raise
@@ -410,6 +418,7 @@ class AdamW(torch.optim.Optimizer):
             if (_sizes(params) != g.numel or _types(params, "AdamW: parameters") != g.types or [p.stride() for p in params] != g.strides
                     or {p.get_device() for p in params} != {self._device.index}):
                 raise RuntimeError("AdamW: a parameter changed its size, type, order or device after the optimizer was made")
+            _check_apart(params)
             g.pointers, g.aliases = ptrs, [p.detach() for p in params]
         return ptrs
 

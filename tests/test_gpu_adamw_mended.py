@@ -158,3 +158,26 @@ def test_a_state_that_does_not_fit_changes_nothing(bits):
     opt.load_state_dict(saved)
     assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["betas"] == (0.5, 0.75)
     opt.step()
+
+
+def test_parameters_that_share_memory_are_refused():
+    """Waves would update the shared elements at the same time, in no order."""
+    import myria3d_amd
+
+    flat = torch.zeros(1000, device="cuda")
+    a, b, c = (flat[i:j].requires_grad_() for i, j in ((0, 500), (500, 1000), (499, 600)))
+    opt = myria3d_amd.AdamW([a, b, torch.zeros(0, device="cuda", requires_grad=True)], lr=0.5)  # neighbours are none
+    tied = flat.view(10, 100).requires_grad_()
+    for bad in ([a, c], [c, b], [tied, b], [tied, flat[:1000].view(10, 100).requires_grad_()]):
+        with pytest.raises(ValueError, match="share"):
+            myria3d_amd.AdamW(bad)
+        with pytest.raises(ValueError, match="share"):
+            opt.add_param_group({"params": [t.detach().requires_grad_() for t in bad]})  # (views of the same memory)
+    assert len(opt.param_groups) == 1
+    b.data = flat[400:900]
+    with pytest.raises(ValueError, match="share"):
+        opt.step()
+    b.data = flat[500:]
+    a.grad, b.grad = torch.ones(500, device="cuda"), -torch.ones(500, device="cuda")
+    opt.step()
+    assert bool((flat[:500] < -0.4).all()) and bool((flat[500:] > 0.4).all())
