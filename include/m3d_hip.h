@@ -521,7 +521,8 @@ int m3d_zero_bump(void* buf, int64_t nbytes, int64_t* counters, int32_t ncounter
 
 /* ---- layer norm ------------------------------------------------------------------------------------------------
  * torch.nn.LayerNorm over the last dimension, with the LeakyReLU that follows a SharedMLP's normalisation
- * (pyg_randla_net.py:92-109 has batch norm there; PyG's MLP takes norm="layer_norm"):
+ * (pyg_randla_net.py:92-109 has batch norm there).  PyG's LayerNorm is this with mode="node"; its default, mode="graph", which
+ * MLP's norm="layer_norm" takes, normalises a cloud as a whole and is another operator:
  *   mean, var over the row;  z = (x - mean) / sqrt(var + eps) * w + b;  y = z > 0 ? z : slope * z   (slope = 1: none)
  * x: [rows, cols], row stride ldx elements (0: the same row again); y contiguous; type: of x and y, wtype: of w and b
  * (nullable: ones, zeros).  mean: fp32 [rows][2], a row's mean as the sum of two floats (one alone has too few digits where
@@ -540,7 +541,8 @@ int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
  * The reference trains through Lightning, whose gradient_clip_val and torch optimizers loop over the parameter tensors.
  * `grads`, `numel`, `types` (and the arrays of M3DAdamW) are HOST arrays of `count` entries read during the call: device
  * pointer of a contiguous tensor (grads: NULL = the tensor has no gradient; aligned to its element, no more), number of
- * elements, type (M3D_TYPE_*).  Any count; the pointers travel as kernel arguments, 152 tensors a launch. */
+ * elements, type (M3D_TYPE_*).  No two tensors that a call writes may share memory.  Any count; the pointers travel as kernel
+ * arguments, 152 tensors a launch. */
 #define M3D_GRAD_NORM_PARTS 2048
 /* parts (device fp64 [M3D_GRAD_NORM_PARTS]) <- partial sums of g^2 over all tensors, *nparts (host) <- how many of them are
  * written: the norm is the root of their sum, which m3d_clip_grads and m3d_adamw_step take themselves.  No atomics: the

@@ -36,7 +36,9 @@ class _LayerNormHolder(nn.Module):
 
 class SharedMLPParams(nn.Module):
     """Parameters of ``SharedMLP(channels, ...)`` (pyg_randla_net.py:97-109).  ``layer_norm``: every point's channels are
-    normalised by themselves (PyG MLP's ``norm="layer_norm"``) instead of every channel over the batch."""
+    normalised by themselves (``torch.nn.LayerNorm``) instead of every channel over the batch.  Of PyG's ``LayerNorm`` that is
+    ``mode="node"``, not the default that its ``MLP(norm="layer_norm")`` takes (one mean and variance a cloud); parity with PyG is
+    unpinned.  The parameters keep the names of this repository's batch norm (``norms.i.module.weight``), not PyG's."""
 
     def __init__(self, channels: Sequence[int], act: bool = True, norm: bool = True, bias: bool = True,
                  dropout: Optional[Sequence[float]] = None, layer_norm: bool = False):

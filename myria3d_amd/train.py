@@ -243,7 +243,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     ``min(1, max_norm / (norm + 1e-6))`` and returns the norm they had together, a 0-dim fp32 tensor on their device (nothing is
     read back).  fp32, bf16 and fp16 gradients, mixed as they come, on one device; parameters without one are left out.  The norm
     is summed in 64 bits in a fixed order: the same gradients give the same bits.  Gradients that are not finite scale as in
-    torch (an infinite norm: zeros, NaN for the infinite ones themselves; a NaN norm: NaN)."""
+    torch (an infinite norm: zeros, NaN for the infinite ones themselves; a NaN norm: NaN).  No two gradients may share memory."""
     params = [parameters] if isinstance(parameters, Tensor) else list(parameters)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -342,8 +342,8 @@ class AdamW(torch.optim.Optimizer):
     becomes zero.  A value that is not finite is held as NaN, in its own element only.
 
     ``max_grad_norm``: the gradients of ALL parameters are taken as ``clip_grad_norm_`` would leave them (``p.grad`` itself is
-    not written); ``grad_norm`` is then the norm they had, a 0-dim fp32 tensor on the device.  A step whose norm is not finite
-    changes nothing and is not counted.
+    not written); ``grad_norm`` is then the norm they had, a 0-dim fp32 tensor on the device, which every step writes again
+    (``clone()`` it to keep one).  A step whose norm is not finite changes nothing and is not counted.
 
     ``lr`` may be a 0-dim fp32 tensor on the device (a schedule under graph replay).  Nothing is read back and step counts live on the
     device: ``step()`` may be captured into a hipGraph (after one eager step) and replayed; the gradients must then be written in
