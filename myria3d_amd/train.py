@@ -463,7 +463,7 @@ class AdamW(torch.optim.Optimizer):
                 for g, (_, ptrs) in zip(self._groups[1:], pointers[1:]):
                     numel, types, grads = numel + g.numel, types + g.types, grads + ptrs
                 call("m3d_grad_norm", _at(grads), _at(numel), _at(types), len(grads), self._parts.data_ptr(), ctypes.addressof(nparts), st)
-            for g, group, (params, ptrs) in zip(self._groups, self.param_groups, pointers):
+            for g, group, (params, ptrs), there in zip(self._groups, self.param_groups, pointers, keep):
                 if not g.params:
                     continue
                 lr, (b1, b2) = group["lr"], group["betas"]
@@ -479,7 +479,7 @@ class AdamW(torch.optim.Optimizer):
                 call("m3d_adamw_step", ctypes.addressof(a), st)
                 # (these parameters changed behind torch's back: graphs and caches that go by their version counters notice.  Whether a
                 # clipped step was taken only the device knows: its parameters count as changed)
-                torch.autograd.graph.increment_version(g.params if all(ptrs) else [p for p, x in zip(g.params, ptrs) if x])
+                torch.autograd.graph.increment_version(g.params if len(there) == len(ptrs) else [p for p, x in zip(g.params, ptrs) if x])
         return loss
 
     # ------------------------------------------------------------------------------------------
