@@ -495,38 +495,41 @@ __global__ __launch_bounds__(1024) void layer_norm_wide_bwd_kernel(const NormArg
   }
 }
 
-// dw and db: the partial rows added up in 64 bits.  16 columns (64 bytes) a workgroup, 64 of its threads to a column.
+// dw and db: the partial rows added up in 64 bits.  16 columns (64 bytes) a workgroup at a time, 64 of its threads to a column.
 __global__ __launch_bounds__(1024) void layer_norm_wgrad_kernel(const float* __restrict__ parts, int nparts, int cols, int wtype,
                                                                 void* __restrict__ dw, void* __restrict__ db) {
   __shared__ double red[64][17];
-  const int tc = threadIdx.x & 15, tr = threadIdx.x >> 4, c = blockIdx.x * 16 + tc;
+  const int tc = threadIdx.x & 15, tr = threadIdx.x >> 4;
   const int64_t ld = 2 * (int64_t)cols;
-  double s = 0.0;
-  if (c < ld) {
-    int p = tr;
-    for (; p + 3 * 64 < nparts; p += 4 * 64) {
-      float v[4];
+  for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < ld; c0 += (int64_t)gridDim.x * 16) {
+    const int64_t c = c0 + tc;
+    double s = 0.0;
+    if (c < ld) {
+      int p = tr;
+      for (; p + 3 * 64 < nparts; p += 4 * 64) {
+        float v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = parts[(p + u * 64) * ld + c];
+        for (int u = 0; u < 4; ++u) v[u] = parts[(p + u * 64) * ld + c];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s += (double)v[u];
+        for (int u = 0; u < 4; ++u) s += (double)v[u];
+      }
+      for (; p < nparts; p += 64) s += (double)parts[p * ld + c];
     }
-    for (; p < nparts; p += 64) s += (double)parts[p * ld + c];
-  }
-  red[tr][tc] = s;
-  __syncthreads();
-  for (int h = 32; h > 0; h >>= 1) {
-    if (tr < h) red[tr][tc] += red[tr + h][tc];
+    red[tr][tc] = s;
     __syncthreads();
-  }
-  if (tr == 0 && c < ld) {
-    void* out = c < cols ? dw : db;
-    const int k = c < cols ? c : c - cols;
-    const float v = (float)red[0][tc];
-    if (!out) return;
-    if (wtype == M3D_TYPE_F32) el_store<M3D_TYPE_F32>(out, k, v);
-    else if (wtype == M3D_TYPE_BF16) el_store<M3D_TYPE_BF16>(out, k, v);
-    else el_store<M3D_TYPE_F16>(out, k, v);
+    for (int h = 32; h > 0; h >>= 1) {
+      if (tr < h) red[tr][tc] += red[tr + h][tc];
+      __syncthreads();
+    }
+    if (tr == 0 && c < ld) {  // (red[0][tc] is this thread's own: no barrier before the next columns)
+      void* out = c < cols ? dw : db;
+      const int64_t k = c < cols ? c : c - cols;
+      const float v = (float)red[0][tc];
+      if (!out) continue;
+      if (wtype == M3D_TYPE_F32) el_store<M3D_TYPE_F32>(out, k, v);
+      else if (wtype == M3D_TYPE_BF16) el_store<M3D_TYPE_BF16>(out, k, v);
+      else el_store<M3D_TYPE_F16>(out, k, v);
+    }
   }
 }
 
@@ -662,7 +665,9 @@ extern "C" int m3d_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, i
     if (rc != M3D_OK) return rc;
   }
   if (dw || db) {  // (no rows: no parts, zeros)
-    hipLaunchKernelGGL(layer_norm_wgrad_kernel, dim3((unsigned)m3d_cdiv(2 * (int64_t)cols, 16)), dim3(1024), 0, st, (const float*)ws,
+    // (a launch has less than 2^32 threads)
+    const int64_t groups = m3d_cdiv(2 * (int64_t)cols, 16), most = 1 << 20;
+    hipLaunchKernelGGL(layer_norm_wgrad_kernel, dim3((unsigned)(groups < most ? groups : most)), dim3(1024), 0, st, (const float*)ws,
                        (int)grid, cols, wtype, dw, db);
     M3D_CHECK_LAUNCH();
   }

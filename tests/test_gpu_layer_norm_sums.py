@@ -67,3 +67,8 @@ def test_few_rows(cols):
 
 def test_every_row_beyond_32_bits():
     whole((1 << 31) // 1024 + 1000, 1024, BF16, None, seed=3)
+
+
+def test_more_columns_than_a_launch_has_threads_for():
+    """One column takes 64 threads in the sums over the partial rows: from 2^25 columns on they pass 2^32."""
+    whole(3, (1 << 25) + 6, BF16, 0.5, seed=4)
