@@ -259,6 +259,8 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
     dense = grads
     if not all(map(Tensor.is_contiguous, grads)):
         _check_strided(grads)
+        if any(stride == 0 and size > 1 for g in grads for size, stride in zip(g.shape, g.stride())):
+            raise RuntimeError("clip_grad_norm_: a gradient whose elements share memory cannot be scaled in place")
         dense = [g if _dense(g) else g.contiguous() for g in grads]
     ptrs, numel = _pointers(dense), _sizes(dense)
     if len(set(ptrs)) < len(ptrs) and len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads):
