@@ -17,13 +17,13 @@
 // a multiple of a vector, one element of the rest.  Up to 64 lanes the row sits inside a wave (narrow rows: several rows a wave,
 // sums by lane swaps, no LDS); above, a workgroup of 128 to 1 024 threads takes a row (sums over its waves through LDS).  The
 // columns of a lane are the same for every row it meets: w and b are read once per lane (where they fit), and the backward pass
-// keeps dw and db of its columns in registers over all its rows.  At the end the waves of a workgroup are added up through LDS in a
-// fixed order, the workgroups leave one row of partial sums each, and a second kernel adds these in 64 bits: no atomics, the same bits
-// every time.
+// keeps dw and db of its columns in registers over all its rows (in 32 bits: at 1.6 M x 64 a lane meets 100 rows and the sums are
+// off by 2e-7; 64 bits would take twice the registers).  At the end the waves of a workgroup are added up through LDS in a fixed order,
+// the workgroups leave one row of partial sums each, and a second kernel adds these in 64 bits: no atomics, the same bits every time.
 // Vectors are loaded with the alignment of their element, so rows of any stride take this path.
 //
-// Bound by memory (6.1 TB/s is what a large scaling reaches here): 1 638 400 x 64 fp32 forward 147 us, 5.7 TB/s, backward 203 + 5 us,
-// 6.1 TB/s; 8 192 x 8 192 bf16 52 us, 5.2 TB/s, and 76 + 7 us, 4.9 TB/s.  The next row's loads are issued before the present row's
+// Bound by memory (6.1 TB/s is what a large scaling reaches here): 1 638 400 x 64 fp32 forward 147 us, 5.7 TB/s, backward 207 + 5 us,
+// 6.0 TB/s; 8 192 x 8 192 bf16 54 us, 5.0 TB/s, and 75 + 7 us, 4.9 TB/s.  The next row's loads are issued before the present row's
 // sums: without that the latter took 74 and 118 us.
 #include "m3d_common.h"
 #include "../../include/m3d_hip.h"
@@ -558,7 +558,7 @@ static int norm_per(const NormShape& s) { return s.tpr && s.tpr <= 64 ? 256 / s.
 // Workgroups: at most 16 waves on each of the 256 compute units (8 in the backward pass with several rows a wave, whose registers
 // allow little more and whose ends, w, b, dw and db, cost more than they hide: 241 against 259 us at 1.6 M x 64 fp32), each with
 // the same number of turns.  Rows of up to 40 bytes: what the registers allow, since only many waves keep some of them in flight (20 M x 3
-// fp32, both passes: 882 -> 555 us, 12 M x 7: 661 -> 533; but 6 M x 15: 450 -> 556).
+// fp32, both passes: 882 -> 547 us, 12 M x 7: 661 -> 533; but 6 M x 15: 450 -> 556).
 static int64_t norm_grid(const NormShape& s, int64_t rows, int32_t cols, int32_t type, bool bwd) {
   const bool few = cols <= (type == M3D_TYPE_F32 ? 10 : 20);
   const int per_unit = few ? (bwd ? 5 : 8) : bwd && s.threads == 256 && norm_per(s) > 1 ? 2 : 1024 / s.threads;

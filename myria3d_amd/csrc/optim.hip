@@ -440,8 +440,8 @@ __device__ __forceinline__ void raw_values(const Raw& r, int type, float (&v)[4]
 //   32 bits: bound by memory.  The next block is on its way while the present one is computed (320 us without).  75 M bf16 parameters
 //     (22 bytes each): 270 us, 6.1 TB/s, what a large scaling reaches here; 3 M fp32 (28 bytes): 19.5 us.
 //   8 bits: 85 vector instructions an element, a third of them in 64 bits, beside 16 bytes: the vector units are busy 71 % of the
-//     time (SQ counters) and 100 M fp32 parameters take 350 us, 4.6 TB/s.  Six or seven waves on a SIMD instead of five change
-//     nothing; fetching ahead costs more in registers than it hides (389 us).
+//     time (SQ counters) and 100 M fp32 parameters take 340 us, 4.7 TB/s; 100 M bf16, 10 bytes an element, 333 us.  Six or seven waves
+//     on a SIMD instead of five change nothing; fetching ahead costs more in registers than it hides (389 us).
 // ONCE: past the caches (see M3D_CACHE_BYTES), but for what is written of the parameters, which the forward pass reads next.
 template <int BITS, bool ONCE>
 __global__ __launch_bounds__(256, 5) void adamw_kernel(const TensorList L, const AdamArgs A) {
