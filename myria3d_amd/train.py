@@ -350,7 +350,8 @@ class AdamW(torch.optim.Optimizer):
     ``lr`` may be a 0-dim fp32 tensor on the device (a schedule under graph replay).  Nothing is read back and step counts live on the
     device: ``step()`` may be captured into a hipGraph (after one eager step) and replayed; the gradients must then be written in
     place.  ``state_dict()`` has torch's layout (``step``, ``exp_avg``, ``exp_avg_sq`` per parameter), and with 32 bits states travel
-    to and from ``torch.optim.AdamW`` and, without a weight decay of its own kind, ``Adam``; with 8 bits the codes and scales are stored, and 32-bit states are taken in too."""
+    to and from ``torch.optim.AdamW`` and, without a weight decay of its own kind, ``Adam``; with 8 bits the codes and scales are
+    stored, and 32-bit states are taken in too."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, max_grad_norm: Optional[float] = None):
@@ -540,7 +541,7 @@ class AdamW(torch.optim.Optimizer):
                 if e:
                     self._check_entry(p, e, True in coded)
             # (everything in the group, as torch does: a scheduler made after this looks for initial_lr)
-            values = {k: tuple(map(float, v)) if k == "betas" else float(v) if isinstance(v, Tensor) else copy.deepcopy(v)
+            values = {k: tuple(map(float, v)) if k == "betas" else float(v) if isinstance(v, Tensor) and v.numel() == 1 else copy.deepcopy(v)
                       for k, v in group.items() if k not in ("params", "decoupled_weight_decay") and not (k == "param_names" and k in mine)}
             self._check_group({**mine, **values})
             todo.append((g, mine, values, entries, True in coded))

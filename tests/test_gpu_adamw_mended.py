@@ -181,3 +181,16 @@ def test_parameters_that_share_memory_are_refused():
     a.grad, b.grad = torch.ones(500, device="cuda"), -torch.ones(500, device="cuda")
     opt.step()
     assert bool((flat[:500] < -0.4).all()) and bool((flat[500:] > 0.4).all())
+
+
+def test_what_a_user_keeps_in_a_group_travels_too():
+    import myria3d_amd
+
+    p = _param(30, seed=9)
+    opt = myria3d_amd.AdamW([{"params": [p], "name": "head", "mask": torch.arange(5.0)}])
+    opt.step()
+    other = myria3d_amd.AdamW([p])
+    saved = opt.state_dict()
+    other.load_state_dict(saved)
+    group = other.param_groups[0]
+    assert group["name"] == "head" and torch.equal(group["mask"], torch.arange(5.0)) and group["mask"] is not saved["param_groups"][0]["mask"]
